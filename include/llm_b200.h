@@ -100,7 +100,8 @@ LLMB_API int llmb_open_reader(llmb_read_fn read, void *user, uint64_t size, int 
 LLMB_API void llmb_close(llmb_model *m);
 
 /* The message of the last failure on this model; with m == NULL, the last
- * failure of llmb_open / llmb_open_reader on the calling thread.  Never NULL. */
+ * failure on the calling thread of a call that takes no model (llmb_open,
+ * llmb_open_reader, llmb_kv8_*, llmb_logits_control).  Never NULL. */
 LLMB_API const char *llmb_last_error(const llmb_model *m);
 
 /* GPU.Cfg, gpu.go:119. */
@@ -225,6 +226,136 @@ LLMB_API int64_t llmb_get_knob(const char *name);
  * caller synchronises. */
 LLMB_API int llmb_attention_noalloc(const float *q, const float *k_cache, const float *v_cache, int n_pos, int heads,
                                     int kv_heads, int head_dim, int kv_stride, float *out, void *stream);
+
+/* ---- A key/value cache held in 8 bits -------------------------------------
+ *
+ * No counterpart in the reference, whose cache is float32 (gpu.go:509).  Like
+ * llmb_attention_noalloc these calls work on device buffers the caller owns,
+ * allocate nothing, are asynchronous on `stream` (a cudaStream_t of the
+ * current device, NULL for the default stream) and may be captured into a
+ * CUDA graph.  Arguments are checked before any work: NULL or misaligned
+ * pointers, memory of another device, bad sizes are LLMB_ERR_ARG, with a
+ * message from llmb_last_error(NULL); an error pending on the calling thread
+ * is LLMB_ERR_CUDA and stays pending.  What only the GPU knows (lengths,
+ * block numbers, row starts) is checked there: nothing outside the buffers
+ * described here is read or written, whatever these hold.
+ *
+ * The cache is a pool of blocks.  A block holds `block` consecutive positions
+ * of one sequence, for every kv head a tile [block][head_dim] of 8-bit
+ * values, and one float scale for each head: element = value * scale.  Keys
+ * and values are two pools of the same layout; both may lie in one
+ * allocation (block_stride).  A sequence's blocks are listed in its row of a
+ * table, so sequences grow block by block and may share the full blocks of a
+ * common prefix. */
+enum { LLMB_F32 = 0, LLMB_F16 = 1, LLMB_BF16 = 2 };   /* types of rows and logits */
+enum { LLMB_KV8_INT8 = 0, LLMB_KV8_E4M3 = 1 };        /* types of the cache */
+
+typedef struct {
+    void *k, *v;             /* block b at b * block_stride bytes: [kv_heads][block][head_dim]; 16-byte aligned */
+    float *k_scale, *v_scale;/* [n_blocks][kv_heads] */
+    int64_t block_stride;    /* bytes; a multiple of 16, at least kv_heads * block * head_dim */
+    int32_t n_blocks;
+    int32_t block;           /* positions per block: 16, 32, 64 or 128 */
+    int32_t kv_heads;
+    int32_t head_dim;        /* 64 or 128 */
+    int32_t type;            /* LLMB_KV8_INT8 or LLMB_KV8_E4M3 */
+} llmb_kv8_cache;
+
+/* The sequences of one call.  Sequence s has `lens[s]` positions once the
+ * rows of this call are in, and the rows starts[s] .. starts[s+1]-1 (of q, k,
+ * v and out) are its last positions, in order.  A sequence may have no rows
+ * and no positions. */
+typedef struct {
+    const int32_t *lens;     /* device, [n_seq] */
+    const int32_t *tables;   /* device, [n_seq] rows of table_stride block numbers */
+    const int32_t *starts;   /* device, [n_seq + 1], not decreasing; NULL: n_rows / n_seq rows each */
+    int32_t n_seq;           /* 1 .. 65535 */
+    int32_t table_stride;    /* entries of a table row */
+    int32_t n_rows;          /* rows of the call's buffers */
+    int32_t max_new;         /* no sequence has more rows than this; 0: not known (n_rows) */
+    int32_t max_len;         /* no sequence has more positions; 0: not known (table_stride * block) */
+} llmb_kv8_batch;
+
+/* Writes the rows of k and v (n_rows rows of [kv_heads][head_dim] elements
+ * of `type`, row_stride elements apart, 16-byte aligned) into the cache.  Per
+ * block and head, with M = 127 (int8) or 448 (e4m3): a block's first rows
+ * give it the scale a * (1 / M), a their largest magnitude.  Rows that come later
+ * and do not fit (a > M scale) grow the scale by the smallest power of two
+ * that fits, and the values already there are rounded to the new step: all
+ * the roundings of a value together stay within one step, however the rows
+ * came.  (A scale that would grow more than 2^20-fold starts anew at a * (1 / M);
+ * the earlier values are 0 then.)  Values round to nearest even.  An infinity
+ * is stored as M steps and a NaN as 0, neither counts for a; a below 2^-100
+ * is stored as 0.  A sequence's blocks that receive rows must belong to it
+ * alone; blocks outside the table's range or the pool are skipped. */
+LLMB_API int llmb_kv8_append(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *k, const void *v,
+                             int type, int64_t row_stride, void *stream);
+
+/* The reverse: the values held at the positions of each sequence's rows,
+ * value * scale rounded once to `type`, into k and v (either may be NULL).
+ * With lens and row counts of the caller's choice this reads any end of a
+ * sequence, e.g. all of it for llmb_attention_noalloc, whose cache rows these
+ * are.  Rows whose block is not in the pool are set to 0; rows of no sequence
+ * stay as they were. */
+LLMB_API int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, void *k, void *v, int type,
+                           int64_t row_stride, void *stream);
+
+/* Attention of the rows' queries over the cache, after the rows' own keys and
+ * values were appended: out = softmax(scale q k) v over the positions up to
+ * and including the row's own (and, with window > 0, among the last `window`
+ * of those); query head h reads kv head h / (heads / kv_heads).  One row of a
+ * sequence is a decoding step, more are a chunk of its prompt.  q and out:
+ * n_rows rows of [heads][head_dim] elements of `type`, q_stride and
+ * out_stride elements apart, 16-byte aligned; out must not overlap q unless
+ * it is the same buffer with the same stride.  scale 0 means
+ * 1 / sqrt(head_dim).  A row that sees no position becomes 0, one whose query
+ * is not finite NaN; rows of no sequence stay as they were.  `workspace`:
+ * llmb_kv8_attention_workspace bytes of the caller's, 16-byte aligned, not
+ * read before it is written; calls that may overlap on the GPU need their
+ * own.  heads / kv_heads at most 64. */
+LLMB_API int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *q,
+                                int64_t q_stride, void *out, int64_t out_stride, int type, int heads, float scale,
+                                int window, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The bytes of workspace that llmb_kv8_attention needs for these sizes with
+ * any type, scale and window (no pointer is looked at), or -1 where they are
+ * not valid. */
+LLMB_API int64_t llmb_kv8_attention_workspace(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, int heads);
+
+/* ---- Logits between a model's head and the next token ---------------------
+ *
+ * No counterpart in the reference, which takes the largest logit as it is
+ * (kernels_fused.go:271).  Device buffers of the caller's, any of the
+ * controls NULL where it is not used; checks, stream and errors as for the
+ * 8-bit cache. */
+typedef struct {
+    const int32_t *history;      /* [rows] rows of history_stride token ids: the prompt, then the answer so far */
+    const int32_t *history_lens; /* [rows]; NULL: history_stride each */
+    const int32_t *prompt_lens;  /* [rows] how many of them are the prompt; NULL: none */
+    int32_t history_stride;      /* at most 524287 */
+    int32_t n_bias;
+    const float *penalties;      /* [rows][3]: repetition, presence, frequency; NULL: 1, 0, 0 */
+    const int32_t *bias_ids;     /* [n_bias] token ids; of a token's biases the last counts */
+    const float *bias_values;    /* [n_bias] */
+    const int32_t *bias_starts;  /* [rows + 1], not decreasing: row r has the biases starts[r] .. starts[r+1]-1, at
+                                  * most 4095 (later ones do not count); NULL: each row has all n_bias <= 4095 */
+    const uint32_t *mask;        /* [rows] rows of mask_stride words: token v is allowed where bit v % 32 of word v / 32 is 1 */
+    int32_t mask_stride;         /* at least (vocab + 31) / 32 */
+} llmb_logits_ctl;
+
+/* For each row of logits (rows rows of vocab elements of `type`, stride
+ * elements apart) and each token: a token of the history has its logit
+ * divided by `repetition` where it is above 0 and multiplied by it elsewhere;
+ * one that the answer has c > 0 times loses presence and frequency * c; then
+ * its bias is added, and it becomes -inf where the mask does not allow it.
+ * In float32, each operation rounded once.  out (may be logits itself with
+ * the same stride, or NULL) receives the result rounded to `type`; tokens
+ * (may be NULL) per row the first index of the largest float32 result, or -1
+ * where none is above -inf (a NaN is never taken).  Token ids outside the
+ * vocabulary are passed over. */
+LLMB_API int llmb_logits_control(const void *logits, int64_t stride, int type, int rows, int vocab,
+                                 const llmb_logits_ctl *ctl, void *out, int64_t out_stride, int32_t *tokens,
+                                 void *stream);
 
 #ifdef __cplusplus
 }

@@ -32,7 +32,11 @@ OK, ERR_ARG, ERR_IO, ERR_FORMAT, ERR_BOUND, ERR_CONFIG, ERR_TENSOR, ERR_MEMORY, 
 EXPORTS = ("llmb_open", "llmb_open_reader", "llmb_close", "llmb_last_error", "llmb_get_config", "llmb_memory_used",
            "llmb_get_stats", "llmb_generate", "llmb_generate_batch", "llmb_prefill_logits", "llmb_generate_logits",
            "llmb_peek",
-           "llmb_set_layers", "llmb_set_knob", "llmb_get_knob", "llmb_attention_noalloc")
+           "llmb_set_layers", "llmb_set_knob", "llmb_get_knob", "llmb_attention_noalloc", "llmb_kv8_append",
+           "llmb_kv8_read", "llmb_kv8_attention", "llmb_kv8_attention_workspace", "llmb_logits_control")
+
+F32, F16, BF16 = range(3)            # types of rows and logits
+KV8_INT8, KV8_E4M3 = range(2)        # types of the 8-bit cache
 
 
 class LlmError(RuntimeError):
@@ -56,6 +60,23 @@ class _Timing(C.Structure):
                 ("generated", C.c_int32), ("submits", C.c_int64), ("dispatches", C.c_int64),
                 ("record_ms", C.c_double), ("submit_ms", C.c_double), ("gpu_prefill_ms", C.c_double),
                 ("gpu_decode_ms", C.c_double), ("decode_kernel_ms", C.c_double), ("decode_launches", C.c_int64)]
+
+
+class _KV8Cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("block_stride", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("n_blocks", "block", "kv_heads", "head_dim", "type")]
+
+
+class _KV8Batch(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("lens", "tables", "starts")] + \
+               [(n, C.c_int32) for n in ("n_seq", "table_stride", "n_rows", "max_new", "max_len")]
+
+
+class _LogitsCtl(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("history", "history_lens", "prompt_lens")] + \
+               [(n, C.c_int32) for n in ("history_stride", "n_bias")] + \
+               [(n, C.c_void_p) for n in ("penalties", "bias_ids", "bias_values", "bias_starts", "mask")] + \
+               [("mask_stride", C.c_int32)]
 
 
 READ_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64)
@@ -91,6 +112,15 @@ def lib() -> C.CDLL:
         L.llmb_get_knob.argtypes, L.llmb_get_knob.restype = [C.c_char_p], C.c_int64
         L.llmb_attention_noalloc.argtypes = [P, P, P, I, I, I, I, I, P, P]
         L.llmb_attention_noalloc.restype = I
+        Q, F = C.c_int64, C.c_float
+        kv8 = [C.POINTER(_KV8Cache), C.POINTER(_KV8Batch)]
+        L.llmb_kv8_append.argtypes, L.llmb_kv8_append.restype = kv8 + [P, P, I, Q, P], I
+        L.llmb_kv8_read.argtypes, L.llmb_kv8_read.restype = kv8 + [P, P, I, Q, P], I
+        L.llmb_kv8_attention.argtypes = kv8 + [P, Q, P, Q, I, I, F, I, P, Q, P]
+        L.llmb_kv8_attention.restype = I
+        L.llmb_kv8_attention_workspace.argtypes, L.llmb_kv8_attention_workspace.restype = kv8 + [I], Q
+        L.llmb_logits_control.argtypes = [P, Q, I, I, I, C.POINTER(_LogitsCtl), P, Q, P, P]
+        L.llmb_logits_control.restype = I
         _lib = L
     return _lib
 
@@ -266,6 +296,221 @@ class GPU:
         out = np.zeros(n, np.float32)
         self._check(lib().llmb_peek(self._h, name.encode(), _ptr(out), n))
         return out
+
+
+# ---- operators over the caller's device tensors
+#
+# These take tensors of any library whose tensors have data_ptr(), shape,
+# stride() and dtype (torch's do); the tensors must stay alive, and their
+# device current, until the work is done. stream is a cudaStream_t handle
+# (torch.cuda.current_stream().cuda_stream), 0 the default stream.
+#
+# A decoding step's kernels take a few microseconds, so these wrappers check
+# with plain comparisons and build a message only for what they refuse.
+
+_NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": "int8", "float8_e4m3fn": "e4m3", "int32": "int32",
+          "uint32": "int32"}
+_ROWS = (F32, F16, BF16)
+
+
+class _Types(dict):
+    """dtype -> its entry in _NAMES, or None."""
+
+    def __missing__(self, dtype):
+        self[dtype] = t = _NAMES.get(str(dtype).rsplit(".", 1)[-1])
+        return t
+
+
+_TYPES = _Types()
+
+
+def _refuse(msg: str):
+    raise LlmError(ERR_ARG, "llm: " + msg)
+
+
+def _op_check(rc: int) -> None:
+    if rc != OK:
+        raise LlmError(rc, lib().llmb_last_error(None).decode(errors="replace"))
+
+
+def _ints(t, what: str, shape: tuple) -> int:
+    """The address of a contiguous int32 tensor of that shape."""
+    if _TYPES[t.dtype] != "int32" or t.shape != shape or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous int32 tensor of shape {shape}")
+    return t.data_ptr()
+
+
+def _floats(t, what: str, shape: tuple) -> int:
+    if _TYPES[t.dtype] != F32 or t.shape != shape or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous float32 tensor of shape {shape}")
+    return t.data_ptr()
+
+
+class KV8Batch:
+    """The sequences of one call on a KV8Cache (llmb_kv8_batch): lens [n_seq] positions each holds once this call's
+    rows are in, tables [n_seq, entries] its block numbers, starts [n_seq + 1] where its rows begin (None: rows / n_seq
+    each), all int32 on the device. The tensors' contents may change between calls; max_new and max_len (0: not known)
+    bound the rows and the positions of any one sequence."""
+
+    def __init__(self, lens, tables, starts=None, rows: int = 0, max_new: int = 0, max_len: int = 0):
+        if len(tables.shape) != 2 or len(lens.shape) != 1:
+            _refuse("lens must have one dimension, tables two")
+        n, entries = lens.shape[0], tables.shape[1]
+        self._keep = (lens, tables, starts)
+        self.rows = rows
+        self._c = _KV8Batch(_ints(lens, "lens", (n,)), _ints(tables, "tables", (n, entries)),
+                            None if starts is None else _ints(starts, "starts", (n + 1,)),
+                            n, entries, rows, max_new, max_len)
+        self._ref = C.byref(self._c)
+
+
+class KV8Cache:
+    """Keys and values held in 8 bits with a scale for each block of positions and kv head (llmb_kv8_cache): k, v
+    [n_blocks, kv_heads, block, head_dim] of int8 or float8_e4m3fn (blocks may lie any multiple of 16 bytes apart),
+    k_scale, v_scale [n_blocks, kv_heads] float32. The tensors are the caller's."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if len(k.shape) != 4 or k.shape != v.shape:
+            _refuse("k and v must be [n_blocks, kv_heads, block, head_dim]")
+        n, heads, block, hd = k.shape
+        t = _TYPES[k.dtype]
+        if t not in ("int8", "e4m3") or t != _TYPES[v.dtype]:
+            _refuse("k and v must both be int8 or both float8_e4m3fn")
+        for x in (k, v):
+            if tuple(x.stride())[1:] != (block * hd, hd, 1) or x.stride(0) != k.stride(0):
+                _refuse("k and v must be contiguous within a block and have one block stride")
+        scales = [_floats(x, "a scale", (n, heads)) for x in (k_scale, v_scale)]
+        self._keep = (k, v, k_scale, v_scale)
+        self.kv_heads, self.head_dim = heads, hd
+        self._c = _KV8Cache(k.data_ptr(), v.data_ptr(), *scales,
+                            max(k.stride(0), heads * block * hd) if n == 1 else k.stride(0), n, block, heads, hd,
+                            KV8_INT8 if t == "int8" else KV8_E4M3)
+        self._ref = C.byref(self._c)
+        self._lib = lib()
+
+    def _rows(self, batch: KV8Batch, x, what: str, heads: int) -> int:
+        """The element distance of the rows of x [rows, heads, head_dim]."""
+        s, hd = x.stride(), self.head_dim
+        if x.shape != (batch.rows, heads, hd) or s[2] != 1 or (s[1] != hd and heads != 1):
+            _refuse(f"{what} must have shape {(batch.rows, heads, hd)} and be contiguous within a row")
+        return s[0] if batch.rows > 1 else max(s[0], heads * hd)
+
+    def _pair(self, batch: KV8Batch, k, v) -> tuple:
+        """(k's address, v's, their type, their row distance); one of them may be None."""
+        x = v if k is None else k
+        if x is None:
+            _refuse("neither k nor v")
+        t, stride = _TYPES[x.dtype], self._rows(batch, x, "k and v", self.kv_heads)
+        if t not in _ROWS:
+            _refuse("rows must be float32, float16 or bfloat16")
+        if k is None:
+            return None, v.data_ptr(), t, stride
+        if v is None:
+            return k.data_ptr(), None, t, stride
+        if v.dtype != k.dtype or self._rows(batch, v, "k and v", self.kv_heads) != stride:
+            _refuse("k and v must have one type and stride")
+        return k.data_ptr(), v.data_ptr(), t, stride
+
+    def append(self, batch: KV8Batch, k, v, stream: int = 0) -> None:
+        """Writes the rows k, v [rows, kv_heads, head_dim] (llmb_kv8_append)."""
+        if k is None or v is None:
+            _refuse("append needs k and v")
+        kp, vp, t, stride = self._pair(batch, k, v)
+        rc = self._lib.llmb_kv8_append(self._ref, batch._ref, kp, vp, t, stride, stream)
+        if rc:
+            _op_check(rc)
+
+    def read(self, batch: KV8Batch, k=None, v=None, stream: int = 0) -> None:
+        """Reads what is held at the rows' positions into k, v [rows, kv_heads, head_dim] (llmb_kv8_read)."""
+        kp, vp, t, stride = self._pair(batch, k, v)
+        rc = self._lib.llmb_kv8_read(self._ref, batch._ref, kp, vp, t, stride, stream)
+        if rc:
+            _op_check(rc)
+
+    def attention_workspace(self, batch: KV8Batch, heads: int) -> int:
+        """Bytes of workspace for attention() with that many query heads (llmb_kv8_attention_workspace)."""
+        n = self._lib.llmb_kv8_attention_workspace(self._ref, batch._ref, heads)
+        if n < 0:
+            _op_check(ERR_ARG)
+        return n
+
+    def attention(self, batch: KV8Batch, q, out, scale: float = 0.0, window: int = 0, workspace=None,
+                  stream: int = 0) -> None:
+        """Attention of the queries q [rows, heads, head_dim] over the cache into out (llmb_kv8_attention); workspace:
+        a contiguous tensor of attention_workspace() bytes."""
+        if len(q.shape) != 3:
+            _refuse("q must be [rows, heads, head_dim]")
+        heads, t = q.shape[1], _TYPES[q.dtype]
+        if t not in _ROWS or out.dtype != q.dtype:
+            _refuse("q and out must both be float32, float16 or bfloat16")
+        qs, os_ = self._rows(batch, q, "q", heads), self._rows(batch, out, "out", heads)
+        w = n = 0
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                _refuse("workspace must be contiguous")
+            w, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        rc = self._lib.llmb_kv8_attention(self._ref, batch._ref, q.data_ptr(), qs, out.data_ptr(), os_, t, heads, scale,
+                                          window, w or None, n, stream)
+        if rc:
+            _op_check(rc)
+
+
+def logits_control(logits, out=None, tokens=None, history=None, history_lens=None, prompt_lens=None, penalties=None,
+                   bias_ids=None, bias_values=None, bias_starts=None, mask=None, stream: int = 0) -> None:
+    """Penalties for repeated tokens, biases and a grammar's mask on logits [rows, vocab], and the largest that is
+    left (llmb_logits_control): out [rows, vocab] (may be logits), tokens [rows] int32; history [rows, n] int32 with
+    history_lens, prompt_lens [rows] int32; penalties [rows, 3] float32 (repetition, presence, frequency); bias_ids
+    int32 and bias_values float32 [n], with bias_starts [rows + 1] int32 for biases of each row's own; mask
+    [rows, ceil(vocab / 32)] int32, bit 1 where a token is allowed."""
+    shape, dtype = logits.shape, logits.dtype
+    if len(shape) != 2:
+        _refuse("logits must be [rows, vocab]")
+    rows, vocab = shape
+    t, s = _TYPES[dtype], logits.stride()
+    if t not in _ROWS or (s[1] != 1 and vocab != 1):
+        _refuse("logits must be float32, float16 or bfloat16, and contiguous within a row")
+    c = _LogitsCtl()
+    op, os_ = None, 0
+    if out is not None:
+        o = out.stride()
+        if out.dtype != dtype or out.shape != shape or (o[1] != 1 and vocab != 1):
+            _refuse("out must have the type and shape of logits and be contiguous within a row")
+        op, os_ = out.data_ptr(), o[0] if rows > 1 else max(o[0], vocab)
+    if history is not None:
+        if len(history.shape) != 2:
+            _refuse("history must be [rows, n]")
+        n = history.shape[1]
+        h = _ints(history, "history", (rows, n))
+        if history_lens is not None:
+            history_lens = _ints(history_lens, "history_lens", (rows,))
+        if prompt_lens is not None:
+            prompt_lens = _ints(prompt_lens, "prompt_lens", (rows,))
+        if n:  # a history of no tokens is none
+            c.history, c.history_stride, c.history_lens, c.prompt_lens = h, n, history_lens, prompt_lens
+    elif history_lens is not None or prompt_lens is not None:
+        _refuse("lengths without a history")
+    if penalties is not None:
+        c.penalties = _floats(penalties, "penalties", (rows, 3))
+    if bias_ids is not None:
+        n = bias_ids.shape[0]
+        if bias_values is None:
+            _refuse("bias_ids without bias_values")
+        ids, values = _ints(bias_ids, "bias_ids", (n,)), _floats(bias_values, "bias_values", (n,))
+        if bias_starts is not None:
+            bias_starts = _ints(bias_starts, "bias_starts", (rows + 1,))
+        if n:
+            c.n_bias, c.bias_ids, c.bias_values, c.bias_starts = n, ids, values, bias_starts
+    elif bias_values is not None or bias_starts is not None:
+        _refuse("biases without bias_ids")
+    if mask is not None:
+        if len(mask.shape) != 2:
+            _refuse("mask must be [rows, words]")
+        c.mask_stride = mask.shape[1]
+        c.mask = _ints(mask, "mask", (rows, c.mask_stride))
+    rc = lib().llmb_logits_control(logits.data_ptr(), s[0] if rows > 1 else max(s[0], vocab), t, rows, vocab, c, op, os_,
+                                   None if tokens is None else _ints(tokens, "tokens", (rows,)), stream)
+    if rc:
+        _op_check(rc)
 
 
 def NewGPU(path: str, ctx: int = 0, device: int = 0) -> GPU:

@@ -985,6 +985,15 @@ inline Model *M(llmb_model *m) { return reinterpret_cast<Model *>(m); }
 inline const Model *M(const llmb_model *m) { return reinterpret_cast<const Model *>(m); }
 
 }  // namespace
+
+// The message of a failed call without a model (ops.hpp).
+void set_thread_error(const char *msg) noexcept {
+    try {
+        t_open_error = msg;
+    } catch (...) {  // no memory for the message: an older one stays
+    }
+}
+
 }  // namespace llmb
 
 using namespace llmb;

@@ -1,0 +1,748 @@
+// The 8-bit key/value cache: append, read, and attention for few rows
+// (llmb_kv8_append, llmb_kv8_read, llmb_kv8_attention).
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+#include <initializer_list>
+#include <type_traits>
+
+#include "kv8.hpp"
+#include "ops.hpp"
+
+namespace llmb {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ------------------------------------------------------------- append --
+
+template <bool E4M3>
+__host__ __device__ constexpr float kv8_top() { return E4M3 ? 448.f : 127.f; }
+
+constexpr float kFit = 1.f / 4096.f;        // a scale still fits top + kFit steps: the scale a (1 / top) made for a fits a, whatever its roundings
+constexpr float kTiny = 7.888609052e-31f;   // 2^-100
+constexpr float kRestart = 1048576.f;       // 2^20
+
+// Four values to 8 bits: to the nearest, ties to even, saturated; NaN becomes 0.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t kv8_pack(const float (&x)[4], float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float y = __fmul_rn(x[i], inv);
+        y = y == y ? fminf(fmaxf(y, -kv8_top<E4M3>()), kv8_top<E4M3>()) : 0.f;
+        if (E4M3) w |= (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3) << (8 * i);
+        else w |= ((uint32_t)__float2int_rn(y) & 0xffu) << (8 * i);
+    }
+    return w;
+}
+
+// A block's new scale from the largest magnitude a of the rows it receives
+// and the scale s0 of the rows it holds (0: none); old_factor is what the
+// values it holds are multiplied by.
+template <bool E4M3>
+__device__ __forceinline__ float kv8_grow(float a, float s0, float &old_factor) {
+    old_factor = 1.f;
+    if (a < kTiny) return s0;
+    const float fresh = __fmul_rn(a, 1.f / kv8_top<E4M3>());
+    if (s0 == 0.f) return fresh;
+    const float r = __fdiv_rn(a, __fmul_rn(kv8_top<E4M3>() + kFit, s0));
+    if (r <= 1.f) return s0;
+    if (!(r <= kRestart)) {
+        old_factor = 0.f;
+        return fresh;
+    }
+    // the least k with r <= 2^k: r = m 2^e, m in [1, 2), gives e, or e + 1 where m > 1
+    const uint32_t u = __float_as_uint(r);
+    const int k = (int)(u >> 23) - 127 + ((u & 0x7fffffu) != 0);
+    old_factor = __uint_as_float((uint32_t)(127 - k) << 23);
+    return __fmul_rn(s0, __uint_as_float((uint32_t)(127 + k) << 23));
+}
+
+template <class T>
+__device__ __forceinline__ void kv8_unpack(const uint4 &r, float (&x)[16 / sizeof(T)]) {
+    const T *e = reinterpret_cast<const T *>(&r);
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[i] = kv8_float<T>(e[i]);
+}
+
+// One block and kv head of K or V: its new rows are held in registers (U
+// pieces of 16 bytes a thread) between the maximum and the rounding, so they
+// are read once.
+template <class T, bool E4M3, int HD, int U>
+__global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__restrict__ k, const T *__restrict__ v,
+                                                    int64_t row_stride) {
+    constexpr int E = 16 / (int)sizeof(T), PR = HD / E;  // elements of a piece, pieces of a row
+    const int s = blockIdx.z, head = blockIdx.y >> 1;
+    const bool val = blockIdx.y & 1;
+    const Kv8Seq q = kv8_seq(c, s);
+    if (q.n <= 0) return;
+    const int first = max(q.first, 0);
+    const int j = (first >> c.bshift) + blockIdx.x, p0 = j << c.bshift;
+    if (p0 >= q.len) return;
+    const int b = kv8_block(c, s, j);
+    if (b < 0) return;
+    const int lo = max(first - p0, 0), hi = min(q.len - p0, c.block), total = (hi - lo) * PR;
+    const T *src = (val ? v : k) + (int64_t)(q.start + p0 + lo - q.first) * row_stride + head * HD;
+    uint8_t *tile = (val ? c.v : c.k) + b * c.bstride + (int64_t)head * c.block * HD;
+    float *scale = (val ? c.vs : c.ks) + (int64_t)b * c.kvh + head;
+    float s0 = lo > 0 ? *scale : 0.f;
+    uint4 x[U];
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int u = threadIdx.x + i * blockDim.x;
+        if (u < total) x[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)(u / PR) * row_stride + u % PR * E));
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if ((int)(threadIdx.x + i * blockDim.x) < total) {
+            float f[E];
+            kv8_unpack<T>(x[i], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float m = fabsf(f[e]);
+                if (m <= FLT_MAX) a = fmaxf(a, m);
+            }
+        }
+    if (!(s0 > 0.f && s0 <= FLT_MAX)) s0 = 0.f;
+    __shared__ float red[8];
+    for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(kFull, a, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();  // and every thread has read the scale
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) a = fmaxf(a, red[w]);
+    float old;
+    const float sc = kv8_grow<E4M3>(a, s0, old);
+    if (s0 == 0.f) old = 0.f;  // rows without a scale are 0
+    if (threadIdx.x == 0) *scale = sc;
+    const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int u = threadIdx.x + i * blockDim.x;
+        if (u < total) {
+            float f[E];
+            kv8_unpack<T>(x[i], f);
+            uint32_t *dst = reinterpret_cast<uint32_t *>(tile + lo * HD + u * E);
+            if constexpr (E == 4) {
+                *dst = kv8_pack<E4M3>(f, inv);
+            } else {
+                const float f0[4] = {f[0], f[1], f[2], f[3]}, f1[4] = {f[4], f[5], f[6], f[7]};
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(kv8_pack<E4M3>(f0, inv), kv8_pack<E4M3>(f1, inv));
+            }
+        }
+    }
+    if (old != 1.f)
+        for (int u = threadIdx.x; u < lo * HD / 4; u += blockDim.x) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(tile) + u;
+            float f[4];
+            kv8_floats<E4M3>(*w, f);
+            *w = kv8_pack<E4M3>(f, old);
+        }
+}
+
+template <class T, bool E4M3, int HD>
+void append_launch(const Kv8 &c, const void *k, const void *v, int64_t row_stride, int touched, cudaStream_t st) {
+    const dim3 grid(touched, 2 * c.kvh, c.nseq);
+    const int pieces = min(c.max_new, c.block) * HD * (int)sizeof(T) / 16;
+    const T *kp = static_cast<const T *>(k), *vp = static_cast<const T *>(v);
+    // (a block has at most 128 rows: HD sizeof(T) / 32 pieces for each of 256 threads)
+    // the fewest threads that hold the rows with few pieces each: a decoding step's single row needs one warp
+    if (pieces <= 64) k_kv8_append<T, E4M3, HD, 2><<<grid, 32, 0, st>>>(c, kp, vp, row_stride);
+    else if (HD * (int)sizeof(T) <= 128 || pieces <= 1024) k_kv8_append<T, E4M3, HD, 4><<<grid, 256, 0, st>>>(c, kp, vp, row_stride);
+    else k_kv8_append<T, E4M3, HD, HD * (int)sizeof(T) / 32><<<grid, 256, 0, st>>>(c, kp, vp, row_stride);
+}
+
+// --------------------------------------------------------------- read --
+
+// One block and kv head of K or V, four values a thread and step.
+template <class T, bool E4M3, int HD>
+__global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k, T *__restrict__ v,
+                                                  int64_t row_stride) {
+    const int s = blockIdx.z, head = blockIdx.y >> 1;
+    const bool val = blockIdx.y & 1;
+    T *dst = val ? v : k;
+    if (!dst) return;
+    const Kv8Seq q = kv8_seq(c, s);
+    if (q.n <= 0) return;
+    // blocks counted from the one that holds the first row's position, which may be below 0
+    const int j = (q.first >> c.bshift) + (int)blockIdx.x, p0 = j * c.block;
+    if (p0 >= q.len) return;
+    const int b = kv8_block(c, s, j);
+    const int lo = max(q.first - p0, 0), hi = min(q.len - p0, c.block);
+    const uint8_t *tile = (val ? c.v : c.k) + (b < 0 ? 0 : b) * c.bstride + (int64_t)head * c.block * HD;
+    const float sc = b < 0 ? 0.f : (val ? c.vs : c.ks)[(int64_t)b * c.kvh + head];
+    dst += (int64_t)(q.start + p0 - q.first) * row_stride + head * HD;
+    for (int u = lo * (HD / 4) + threadIdx.x; u < hi * (HD / 4); u += blockDim.x) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        if (b >= 0) {
+            kv8_floats<E4M3>(__ldg(reinterpret_cast<const uint32_t *>(tile) + u), f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __fmul_rn(f[i], sc);
+        }
+        T *o = dst + (int64_t)(u / (HD / 4)) * row_stride + u % (HD / 4) * 4;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(o) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+            T h[4] = {kv8_from<T>(f[0]), kv8_from<T>(f[1]), kv8_from<T>(f[2]), kv8_from<T>(f[3])};
+            *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(h);
+        }
+    }
+}
+
+// ---------------------------------------------------------- attention --
+
+constexpr int kAttWarps = 8;
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Attention of a tile of rows of one (sequence, kv head) over one part of the
+// positions: softmax with a running maximum, both products as m16n8k16 with
+// the 8-bit values exact in float16.
+//
+// A warp takes every 8th group of 16 positions, straight from global memory
+// into its registers: the contraction's index may be permuted as long as both
+// operands agree, so lane (g, t) = (lane / 4, lane % 4) loads 16 contiguous
+// bytes of K row g and uses them as its B fragments, and HD / 8 contiguous
+// bytes of the V rows 2t, 2t + 1, 2t + 8, 2t + 9.
+//
+// float32 rows (PIECES = 2) are the sum of two float16 pieces, which hold 22
+// bits of the row's largest element after a power of two has brought it to
+// [2^14, 2^15): the upper 8 rows of a matrix tile are the first pieces, the
+// lower 8 the second, and lane (g, t) holds both results.  The weights go
+// into the second product the same way.  bfloat16 rows fill a tile of 16.
+//
+// The scale of V's block enters the weights' exponent (its power of two, so
+// that the largest weight of all stays near 2^6 and float16 holds the small
+// ones) and mantissa.
+//
+// float16 rows fit one piece, but a weight rounded to float16 is off as much
+// as the result's own rounding, so they take the two-piece form as well.
+template <class T>
+constexpr int kPieces = 2;
+template <>
+constexpr int kPieces<__nv_bfloat16> = 1;
+
+template <class T, bool E4M3, int HD, int PIECES>
+__global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, const Kv8Att a) {
+    constexpr int ROWS = PIECES == 2 ? 8 : 16, NR = PIECES == 2 ? 1 : 2;  // rows of a tile; of a lane
+    constexpr int KS = HD / 16, NT = HD / 8;                              // k steps; column tiles of V
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int s = blockIdx.z, head = blockIdx.y % c.kvh, row0 = blockIdx.y / c.kvh * ROWS;
+    const Kv8Seq sq = kv8_seq(c, s);
+    const int rows = sq.n * a.group;
+    if (row0 >= rows) return;
+    const int last = min(row0 + ROWS, rows) - 1;
+    const int tok0 = row0 / a.group, tok1 = last / a.group;
+    int lo, hi;
+    kv8_span(sq, a.window, tok0, tok1, lo, hi);
+    if (blockIdx.x > 0 && lo + (int64_t)blockIdx.x * a.part >= hi) return;
+    lo += blockIdx.x * a.part;
+    hi = min(hi, lo + a.part);
+
+    // the rows' queries as A fragments
+    uint32_t qf[KS][4];
+    float fac[NR];
+    int pos[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = row0 + g + 8 * i;
+        const bool on = r < rows;
+        const int tok = r / a.group, h = head * a.group + r - tok * a.group;
+        pos[i] = on ? sq.first + tok : -1;
+        const T *qp = static_cast<const T *>(a.q) + (int64_t)(sq.start + (on ? tok : tok0)) * a.q_stride + (on ? h : head * a.group) * HD;
+        float x[KS][4], m = 0.f;
+        bool fine = true;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            // 16 bytes of K hold the 4 values of 4 steps: value e of step ks is element 64 (ks / 4) + 16 t + 4 (ks % 4) + e
+            const T *e = qp + 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
+            T v[4];
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(e);
+            else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(e);
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) {
+                x[ks][e2] = kv8_float<T>(v[e2]);
+                fine = fine && fabsf(x[ks][e2]) <= FLT_MAX;
+                m = fmaxf(m, fabsf(x[ks][e2]));
+            }
+        }
+        m = fmaxf(m, __shfl_xor_sync(kFull, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(kFull, m, 2));
+        fine = __shfl_xor_sync(kFull, (int)fine, 1) && fine;
+        fine = __shfl_xor_sync(kFull, (int)fine, 2) && fine;
+        // m = [1, 2) 2^e becomes [2^14, 2^15); a row that is not finite has NaN as its factor
+        const int ex = fine && m > 0.f ? max(ilogbf(m), -100) : 0;
+        const float up = fine ? scalbnf(1.f, 14 - ex) : 0.f;
+        fac[i] = fine ? a.scale * kv8_unit<E4M3>() * scalbnf(1.f, ex - 14) : NAN;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = fine ? x[ks][e] * up : 0.f;
+            const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
+            qf[ks][i] = h0, qf[ks][2 + i] = h1;
+            if (PIECES == 2) {
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
+                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+                qf[ks][1] = pack_half2(y[0] - f0.x, y[1] - f0.y);
+                qf[ks][3] = pack_half2(y[2] - f1.x, y[3] - f1.y);
+            }
+        }
+    }
+
+    float o[NT][4], m[NR], l[NR];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) m[i] = -FLT_MAX, l[i] = 0.f;
+
+    // a group of 16 positions as a lane holds it
+    struct Group {
+        uint4 k[2][HD / 64];
+        uint32_t v[4][HD / 32];
+        float ks, vs;
+        int b;
+    };
+    auto load = [&](Group &x, int p0) {
+        if (p0 >= hi) {
+            x.b = -1;
+            return;
+        }
+        x.b = kv8_block(c, s, p0 >> c.bshift);
+        if (x.b < 0) return;
+        const int64_t at = x.b * c.bstride + ((int64_t)head * c.block + (p0 & (c.block - 1))) * HD;
+        const uint8_t *kp = c.k + at, *vp = c.v + at;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i)
+                x.k[n][i] = __ldg(reinterpret_cast<const uint4 *>(kp + (8 * n + g) * HD + 64 * i + 16 * t));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint8_t *r = vp + (2 * t + (n & 1) + 8 * (n >> 1)) * HD + g * (HD / 8);
+            if constexpr (HD == 64) {
+                const uint2 w = __ldg(reinterpret_cast<const uint2 *>(r));
+                x.v[n][0] = w.x, x.v[n][1] = w.y;
+            } else {
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(r));
+                x.v[n][0] = w.x, x.v[n][1] = w.y, x.v[n][2] = w.z, x.v[n][3] = w.w;
+            }
+        }
+        x.ks = __ldg(c.ks + (int64_t)x.b * c.kvh + head);
+        x.vs = __ldg(c.vs + (int64_t)x.b * c.kvh + head);
+    };
+    auto use = [&](const Group &x, int p0) {
+        if (x.b < 0) return;
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint4 &w4 = x.k[n][ks / 4];
+                const uint32_t w = ks % 4 == 0 ? w4.x : ks % 4 == 1 ? w4.y : ks % 4 == 2 ? w4.z : w4.w;
+                mma16816(sc[n], qf[ks], kv8_half2<E4M3>(__byte_perm(w, 0, 0x4140)),
+                         kv8_half2<E4M3>(__byte_perm(w, 0, 0x4342)));
+            }
+        }
+        // V's scale = mv 2^lv
+        const bool has = x.vs > 0.f;
+        const int lv = has ? ilogbf(x.vs) : 0;
+        const float mv = has ? scalbnf(x.vs, -lv) : x.vs, flv = (float)lv, unlv = scalbnf(1.f, -lv);
+        float z[NR][4];  // scores in log2, V's exponent added; position 16 + 8 (e / 2) + 2 t + e % 2
+        bool up = false;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const float f = fac[i] * x.ks;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float d = PIECES == 2 ? sc[e >> 1][e & 1] + sc[e >> 1][2 + (e & 1)] : sc[e >> 1][2 * i + (e & 1)];
+                const int p = p0 + 8 * (e >> 1) + 2 * t + (e & 1);
+                const bool seen = p <= pos[i] && p < hi && (a.window == 0 || p > pos[i] - a.window);
+                z[i][e] = seen ? fmaf(d, f, flv) : -INFINITY;
+                up |= z[i][e] - m[i] > 8.f;
+            }
+        }
+        if (__any_sync(kFull, up)) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                float n = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3]));
+                n = fmaxf(n, __shfl_xor_sync(kFull, n, 1));
+                n = fmaxf(n, __shfl_xor_sync(kFull, n, 2));
+                n = fmaxf(n, m[i]);
+                const float r = kv8_exp2(m[i] - n);
+                m[i] = n;
+                l[i] *= r;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    o[j][2 * i] *= r, o[j][2 * i + 1] *= r;
+                    if (PIECES == 2) o[j][2] *= r, o[j][3] *= r;
+                }
+            }
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            float w[4], sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = kv8_exp2(z[i][e] - m[i] + 6.f);
+                sum += w[e];
+                w[e] *= mv;
+            }
+            l[i] = fmaf(sum, unlv, l[i]);
+            pf[i] = pack_half2(w[0], w[1]), pf[2 + i] = pack_half2(w[2], w[3]);
+            if (PIECES == 2) {
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&pf[0]));
+                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&pf[2]));
+                pf[1] = pack_half2(w[0] - f0.x, w[1] - f0.y);
+                pf[3] = pack_half2(w[2] - f1.x, w[3] - f1.y);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j += 4) {
+            // column tiles j .. j + 3 are the 4 bytes of word j / 4 of each V row
+            const uint32_t a0 = __byte_perm(x.v[0][j / 4], x.v[1][j / 4], 0x5140), a1 = __byte_perm(x.v[0][j / 4], x.v[1][j / 4], 0x7362);
+            const uint32_t b0 = __byte_perm(x.v[2][j / 4], x.v[3][j / 4], 0x5140), b1 = __byte_perm(x.v[2][j / 4], x.v[3][j / 4], 0x7362);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t sel = e & 1 ? 0x4342 : 0x4140;
+                mma16816(o[j + e], pf, kv8_half2<E4M3>(__byte_perm(e < 2 ? a0 : a1, 0, sel)),
+                         kv8_half2<E4M3>(__byte_perm(e < 2 ? b0 : b1, 0, sel)));
+            }
+        }
+    };
+
+    Group x0, x1;
+    const int step = 16 * kAttWarps;
+    int p = lo + 16 * warp;
+    load(x0, p);
+    for (; p < hi; p += 2 * step) {
+        load(x1, p + step);
+        use(x0, p);
+        load(x0, p + 2 * step);
+        use(x1, p + step);
+    }
+
+    // the warps' results, joined 64 elements at a time
+    __shared__ float so[kAttWarps][ROWS][64 + 4];
+    __shared__ float2 sml[kAttWarps][ROWS];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        l[i] += __shfl_xor_sync(kFull, l[i], 1);
+        l[i] += __shfl_xor_sync(kFull, l[i], 2);
+        if (t == 0) sml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+    }
+    const int nrow = last - row0 + 1;
+    for (int d0 = 0; d0 < HD; d0 += 64) {
+        if (d0 > 0) __syncthreads();
+        // column tile j's columns 2t, 2t + 1 are elements 2t HD/8 + j and (2t + 1) HD/8 + j
+        const int c0 = 2 * t * (HD / 8) - d0;
+        if (c0 >= 0 && c0 < 64) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        so[warp][g + 8 * i][c0 + e * (HD / 8) + j] = PIECES == 2 ? o[j][e] + o[j][2 + e] : o[j][2 * i + e];
+        }
+        __syncthreads();
+        for (int u = threadIdx.x; u < nrow * 64; u += kAttWarps * 32) {
+            const int r = u / 64, d = u % 64;
+            float M = -FLT_MAX, L = 0.f, O = 0.f;
+#pragma unroll
+            for (int w = 0; w < kAttWarps; ++w) M = fmaxf(M, sml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kAttWarps; ++w) {
+                const float f = kv8_exp2(sml[w][r].x - M);
+                L = fmaf(f, sml[w][r].y, L);
+                O = fmaf(f, so[w][r][d], O);
+            }
+            O *= kv8_unit<E4M3>();
+            const int rr = row0 + r, tok = rr / a.group, h = head * a.group + rr - tok * a.group;
+            if (a.splits == 1) {
+                // no position seen: every warp's sum is 0
+                static_cast<T *>(a.out)[(int64_t)(sq.start + tok) * a.out_stride + h * HD + d0 + d] =
+                    kv8_from<T>(L == 0.f ? 0.f : O / L);
+            } else {
+                const int64_t at = ((int64_t)(sq.start + tok) * a.heads + h) * a.splits + blockIdx.x;
+                a.part_o[at * HD + d0 + d] = O;
+                if (d0 + d == 0) a.part_ml[at] = make_float2(M, L);
+            }
+        }
+    }
+}
+
+// Joins the parts of one (row, query head): a warp each.
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_kv8_join(const Kv8 c, const Kv8Att a) {
+    cudaGridDependencySynchronize();
+    const int lane = threadIdx.x & 31, s = blockIdx.z;
+    const Kv8Seq sq = kv8_seq(c, s);
+    const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    if (r >= (int64_t)sq.n * a.heads) return;
+    const int tok = (int)(r / a.heads), h = (int)(r % a.heads), kvr = tok * a.group + h % a.group;
+    // the span of the row's tile, as its parts were cut
+    const int row0 = kvr / a.tile * a.tile, last = min(row0 + a.tile, sq.n * a.group) - 1;
+    int lo, hi;
+    kv8_span(sq, a.window, row0 / a.group, last / a.group, lo, hi);
+    const int parts = max((hi - lo + a.part - 1) / a.part, 1);
+    const int64_t at = ((int64_t)(sq.start + tok) * a.heads + h) * a.splits;
+    float M = -FLT_MAX;
+    for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.part_ml[at + i].x);
+    for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, k));
+    float L = 0.f, O[HD / 32];
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) O[k] = 0.f;
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = a.part_ml[at + i];
+        const float f = kv8_exp2(ml.x - M);
+        L = fmaf(f, ml.y, L);
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k) O[k] = fmaf(f, a.part_o[(at + i) * HD + lane + 32 * k], O[k]);
+    }
+    T *out = static_cast<T *>(a.out) + (int64_t)(sq.start + tok) * a.out_stride + h * HD;
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) out[lane + 32 * k] = kv8_from<T>(L == 0.f ? 0.f : O[k] / L);
+}
+
+// --------------------------------------------------------------- host --
+
+int esize(int type) { return type == LLMB_F32 ? 4 : 2; }
+
+// The sizes of a cache and a batch (no pointer): LLMB_OK, and what the kernels take.
+int kv8_sizes(const char *what, const llmb_kv8_cache *c, const llmb_kv8_batch *b, Kv8 &k) noexcept {
+    if (!c || !b) return op_error(LLMB_ERR_ARG, "llm: %s: no cache or no batch", what);
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
+        return op_error(LLMB_ERR_ARG, "llm: %s: blocks of %d positions (16, 32, 64 or 128)", what, c->block);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return op_error(LLMB_ERR_ARG, "llm: %s: head_dim %d (64 or 128)", what, c->head_dim);
+    if (c->type != LLMB_KV8_INT8 && c->type != LLMB_KV8_E4M3)
+        return op_error(LLMB_ERR_ARG, "llm: %s: no cache type %d", what, c->type);
+    if (c->kv_heads < 1 || c->kv_heads > 4096 || c->n_blocks < 1)
+        return op_error(LLMB_ERR_ARG, "llm: %s: %d blocks of %d kv heads", what, c->n_blocks, c->kv_heads);
+    if (c->block_stride % 16 != 0 || c->block_stride < (int64_t)c->kv_heads * c->block * c->head_dim)
+        return op_error(LLMB_ERR_ARG, "llm: %s: block_stride %lld", what, (long long)c->block_stride);
+    if (b->n_seq < 1 || b->n_seq > 65535 || b->table_stride < 1 || b->n_rows < 0 || b->max_new < 0 || b->max_len < 0)
+        return op_error(LLMB_ERR_ARG, "llm: %s: %d sequences, %d table entries, %d rows, max_new %d, max_len %d", what,
+                        b->n_seq, b->table_stride, b->n_rows, b->max_new, b->max_len);
+    const int64_t held = (int64_t)b->table_stride * c->block;
+    if (held > INT32_MAX - 4096)
+        return op_error(LLMB_ERR_ARG, "llm: %s: tables of more than 2^31 positions", what);
+    k = Kv8{};
+    k.bstride = c->block_stride, k.nblocks = c->n_blocks, k.block = c->block, k.kvh = c->kv_heads;
+    k.bshift = c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
+    k.nseq = b->n_seq, k.tstride = b->table_stride, k.nrows = b->n_rows;
+    k.max_new = b->max_new > 0 && b->max_new < b->n_rows ? b->max_new : b->n_rows;
+    k.cap = b->max_len > 0 && b->max_len < held ? b->max_len : (int)held;
+    k.k = static_cast<uint8_t *>(c->k), k.v = static_cast<uint8_t *>(c->v);
+    k.ks = c->k_scale, k.vs = c->v_scale;
+    k.lens = b->lens, k.tables = b->tables, k.starts = b->starts;
+    if (!b->starts) {
+        if (b->n_rows % b->n_seq != 0)
+            return op_error(LLMB_ERR_ARG, "llm: %s: %d rows do not divide among %d sequences", what, b->n_rows, b->n_seq);
+        k.max_new = b->n_rows / b->n_seq < k.max_new ? b->n_rows / b->n_seq : k.max_new;
+    }
+    return LLMB_OK;
+}
+
+int kv8_rows(const char *what, int type, int64_t stride, int64_t width) noexcept {
+    if (type != LLMB_F32 && type != LLMB_F16 && type != LLMB_BF16)
+        return op_error(LLMB_ERR_ARG, "llm: %s: no type %d", what, type);
+    if (stride < width || stride * esize(type) % 16 != 0)
+        return op_error(LLMB_ERR_ARG, "llm: %s: rows %lld elements apart (at least %lld, a multiple of 16 bytes)", what,
+                        (long long)stride, (long long)width);
+    return LLMB_OK;
+}
+
+int kv8_pointers(const char *what, int *device, const Kv8 &c, const void *x, const char *nx, const void *y,
+                 const char *ny, bool optional) noexcept {
+    const std::initializer_list<OpPointer> ps = {
+        {c.k, "cache k", 16, false},     {c.v, "cache v", 16, false},   {c.ks, "k_scale", 4, false},
+        {c.vs, "v_scale", 4, false},     {c.lens, "lens", 4, false},    {c.tables, "tables", 4, false},
+        {c.starts, "starts", 4, true},   {x, nx, 16, optional},         {y, ny, 16, optional}};
+    int rc = op_alignment(what, ps);
+    if (rc == LLMB_OK) rc = op_device(what, device);
+    if (rc == LLMB_OK) rc = op_pointers(what, *device, ps);
+    return rc;
+}
+
+// Blocks that n consecutive positions can touch.
+int64_t touched(const Kv8 &c) { return ((int64_t)c.max_new + c.block - 2) / c.block + 1; }
+
+template <class F>
+void by_type(int type, F &&f) {
+    if (type == LLMB_F32) f(float{});
+    else if (type == LLMB_F16) f(__half{});
+    else f(__nv_bfloat16{});
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+template <class F>
+void by_cache(int type, int hd, F &&f) {
+    if (type == LLMB_KV8_E4M3) hd == 64 ? f(Yes{}, std::integral_constant<int, 64>{}) : f(Yes{}, std::integral_constant<int, 128>{});
+    else hd == 64 ? f(No{}, std::integral_constant<int, 64>{}) : f(No{}, std::integral_constant<int, 128>{});
+}
+
+// How the attention cuts its work: rows into tiles, a tile's positions into parts.
+struct Cut {
+    int tile, tiles, splits, part;
+    int most;  // splits is never more, and it does not shrink with the window
+};
+
+Cut attention_cut(const Kv8 &c, int heads, int tile, int window) {
+    Cut k{};
+    const int group = heads / c.kvh;
+    k.tile = tile;
+    k.tiles = (int)(((int64_t)c.max_new * group + tile - 1) / tile);
+    int64_t span = c.cap;
+    if (window > 0 && window < c.cap) {
+        const int64_t tokens = std::min<int64_t>(c.max_new, (tile + group - 2) / group + 1);
+        span = std::min<int64_t>(span, (int64_t)window + tokens + 15);
+    }
+    const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
+    int64_t want = (2 * 148 + units - 1) / units;
+    const int64_t most = std::max<int64_t>(span / 512, 1);  // a part is worth a launch's join from 512 positions on
+    want = std::max<int64_t>(1, std::min<int64_t>({want, most, 64}));
+    k.most = (int)want;
+    k.part = (int)((span + want - 1) / want + 127) / 128 * 128;
+    k.splits = (int)((span + k.part - 1) / k.part);
+    if (k.splits < 1) k.splits = 1;
+    return k;
+}
+
+}  // namespace
+}  // namespace llmb
+
+using namespace llmb;
+
+extern "C" {
+
+int llmb_kv8_append(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *k, const void *v, int type,
+                    int64_t row_stride, void *stream) {
+    const char *what = "kv8_append";
+    Kv8 c;
+    int rc = kv8_sizes(what, cache, batch, c);
+    if (rc == LLMB_OK) rc = kv8_rows(what, type, row_stride, (int64_t)c.kvh * cache->head_dim);
+    int dev = 0;
+    if (rc == LLMB_OK) rc = kv8_pointers(what, &dev, c, k, "k", v, "v", c.nrows == 0);
+    if (rc != LLMB_OK) return rc;
+    if (c.max_new == 0) return LLMB_OK;
+    by_type(type, [&](auto t) {
+        by_cache(cache->type, cache->head_dim, [&](auto e4m3, auto hd) {
+            append_launch<decltype(t), decltype(e4m3)::value, decltype(hd)::value>(
+                c, k, v, row_stride, (int)touched(c), static_cast<cudaStream_t>(stream));
+        });
+    });
+    return op_launched(what);
+}
+
+int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, void *k, void *v, int type,
+                  int64_t row_stride, void *stream) {
+    const char *what = "kv8_read";
+    Kv8 c;
+    int rc = kv8_sizes(what, cache, batch, c);
+    if (rc == LLMB_OK) rc = kv8_rows(what, type, row_stride, (int64_t)c.kvh * cache->head_dim);
+    int dev = 0;
+    if (rc == LLMB_OK) rc = kv8_pointers(what, &dev, c, k, "k", v, "v", true);
+    if (rc != LLMB_OK) return rc;
+    if (c.max_new == 0 || (!k && !v)) return LLMB_OK;
+    by_type(type, [&](auto t) {
+        by_cache(cache->type, cache->head_dim, [&](auto e4m3, auto hd) {
+            using T = decltype(t);
+            k_kv8_read<T, decltype(e4m3)::value, decltype(hd)::value>
+                <<<dim3((unsigned)touched(c), 2 * c.kvh, c.nseq), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                    c, static_cast<T *>(k), static_cast<T *>(v), row_stride);
+        });
+    });
+    return op_launched(what);
+}
+
+int64_t llmb_kv8_attention_workspace(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, int heads) {
+    Kv8 c;
+    if (kv8_sizes("kv8_attention_workspace", cache, batch, c) != LLMB_OK) return -1;
+    if (heads < 1 || heads % c.kvh != 0 || heads / c.kvh > kKv8MaxGroup) {
+        op_error(LLMB_ERR_ARG, "llm: kv8_attention_workspace: %d heads on %d kv heads", heads, c.kvh);
+        return -1;
+    }
+    int splits = 1;
+    for (int tile : {8, 16}) splits = std::max(splits, attention_cut(c, heads, tile, 0).most);
+    return splits == 1 ? 0 : (int64_t)c.nrows * heads * splits * (8 + 4 * (int64_t)cache->head_dim);
+}
+
+int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *q, int64_t q_stride,
+                       void *out, int64_t out_stride, int type, int heads, float scale, int window, void *workspace,
+                       int64_t workspace_bytes, void *stream) {
+    const char *what = "kv8_attention";
+    Kv8 c;
+    int rc = kv8_sizes(what, cache, batch, c);
+    if (rc != LLMB_OK) return rc;
+    const int hd = cache->head_dim;
+    if (heads < 1 || heads % c.kvh != 0 || heads / c.kvh > kKv8MaxGroup)
+        return op_error(LLMB_ERR_ARG, "llm: %s: %d heads on %d kv heads", what, heads, c.kvh);
+    if (window < 0 || !(std::fabs(scale) <= FLT_MAX))
+        return op_error(LLMB_ERR_ARG, "llm: %s: window %d, scale %g", what, window, (double)scale);
+    if ((rc = kv8_rows(what, type, q_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
+    if ((rc = kv8_rows(what, type, out_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
+    int dev = 0;
+    if ((rc = kv8_pointers(what, &dev, c, q, "q", out, "out", c.nrows == 0)) != LLMB_OK) return rc;
+    if (c.max_new == 0) return LLMB_OK;
+    Kv8Att a{};
+    const Cut cut = attention_cut(c, heads, type == LLMB_BF16 ? 16 : 8, window);
+    if ((int64_t)c.kvh * cut.tiles > 65535)
+        return op_error(LLMB_ERR_ARG, "llm: %s: %d rows of a sequence are too many", what, c.max_new);
+    const int64_t slots = (int64_t)c.nrows * heads * cut.splits;
+    if (cut.splits > 1) {
+        const std::initializer_list<OpPointer> ps = {{workspace, "workspace", 16, false}};
+        if ((rc = op_alignment(what, ps)) != LLMB_OK || (rc = op_pointers(what, dev, ps)) != LLMB_OK) return rc;
+        if (workspace_bytes < slots * (8 + 4 * (int64_t)hd))
+            return op_error(LLMB_ERR_ARG, "llm: %s: a workspace of %lld bytes (llmb_kv8_attention_workspace says %lld)",
+                            what, (long long)workspace_bytes, (long long)(slots * (8 + 4 * (int64_t)hd)));
+        a.part_o = static_cast<float *>(workspace);
+        a.part_ml = reinterpret_cast<float2 *>(a.part_o + slots * hd);
+    }
+    a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+    a.heads = heads, a.group = heads / c.kvh, a.window = window;
+    a.scale = (float)((scale != 0.f ? (double)scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
+    a.tile = cut.tile, a.splits = cut.splits, a.part = cut.part;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    by_type(type, [&](auto t) {
+        by_cache(cache->type, hd, [&](auto e4m3, auto d) {
+            using T = decltype(t);
+            constexpr int HD = decltype(d)::value;
+            k_kv8_attend<T, decltype(e4m3)::value, HD, kPieces<T>>
+                <<<dim3(cut.splits, c.kvh * cut.tiles, c.nseq), kAttWarps * 32, 0, st>>>(c, a);
+        });
+    });
+    if ((rc = op_launched(what)) != LLMB_OK || cut.splits == 1) return rc;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)(((int64_t)c.max_new * heads + 7) / 8), 1, c.nseq);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st, cfg.attrs = &attr, cfg.numAttrs = 1;
+    by_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (hd == 64) cudaLaunchKernelEx(&cfg, k_kv8_join<T, 64>, c, a);
+        else cudaLaunchKernelEx(&cfg, k_kv8_join<T, 128>, c, a);
+    });
+    return op_launched(what);
+}
+
+}  // extern "C"
