@@ -15,8 +15,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllmb200.so")
-SOURCES = ["gguf.cpp", "kernels.cu", "gemm.cu", "decode.cu", "engine.cu", "noalloc.cu", "ops.cpp", "kv8.cu", "logits.cu"]
-HEADERS = ["gguf.hpp", "device.hpp", "kernels.hpp", "ops.hpp", "kv8.hpp", os.path.join("..", "..", "include", "llm_b200.h")]
+SOURCES = ["gguf.cpp", "kernels.cu", "gemm.cu", "decode.cu", "engine.cu", "noalloc.cu", "ops.cpp", "kv8.cu", "kv8_chunk.cu", "logits.cu"]
+HEADERS = ["gguf.hpp", "device.hpp", "kernels.hpp", "ops.hpp", "kv8.hpp", "kv8_chunk.hpp", os.path.join("..", "..", "include", "llm_b200.h")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", os.path.join(ROOT, "include")]
 # The persistent decode kernel's launch bounds still set its register budget; with this flag ptxas allocates

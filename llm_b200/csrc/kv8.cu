@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "kv8.hpp"
+#include "kv8_chunk.hpp"
 #include "ops.hpp"
 
 namespace llmb {
@@ -601,29 +602,63 @@ void by_cache(int type, int hd, F &&f) {
 
 // How the attention cuts its work: rows into tiles, a tile's positions into parts.
 struct Cut {
+    bool chunk;  // by the kernel for many rows
     int tile, tiles, splits, part;
-    int most;  // splits is never more, and it does not shrink with the window
 };
 
-Cut attention_cut(const Kv8 &c, int heads, int tile, int window) {
+// Parts of the kernel for many rows: one CTA takes an SM, so with `units` CTAs of one part each the last wave may be
+// nearly empty; parts fill it, at the price of the join.  Measured on a B200: a step of 128 positions 3 us, a CTA's start
+// 4 us, the join 3 us and its traffic at 4 TB/s.
+int chunk_parts(int64_t units, int64_t span, int64_t slots, int hd) {
+    const int64_t steps = (span + 127) / 128;
+    int best = 1;
+    double least = 0;
+    for (int s = 1; s <= 64 && s <= steps; ++s) {
+        const double waves = (double)((units * s + 147) / 148);
+        const double us = waves * (3.0 * (double)((steps + s - 1) / s) + 4.0) + (s > 1 ? 3.0 + (double)slots * s * hd * 8 / 4e6 : 0.0);
+        if (s == 1 || us < least) least = us, best = s;
+    }
+    return best;
+}
+
+Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     Cut k{};
     const int group = heads / c.kvh;
+    const int64_t rows = (int64_t)c.max_new * group;
+    // rows of one kv head from which on the tensor cores' tiles pay
+    k.chunk = rows > 64;
+    const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 ? 16 : 8;
     k.tile = tile;
-    k.tiles = (int)(((int64_t)c.max_new * group + tile - 1) / tile);
-    int64_t span = c.cap;
-    if (window > 0 && window < c.cap) {
+    k.tiles = (int)((rows + tile - 1) / tile);
+    // the most positions that a tile's rows see between them
+    auto span_of = [&](int w) -> int64_t {
+        if (w <= 0 || w >= c.cap) return c.cap;
         const int64_t tokens = std::min<int64_t>(c.max_new, (tile + group - 2) / group + 1);
-        span = std::min<int64_t>(span, (int64_t)window + tokens + 15);
-    }
+        return std::min<int64_t>(c.cap, (int64_t)w + tokens + 15);
+    };
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
-    int64_t want = (2 * 148 + units - 1) / units;
-    const int64_t most = std::max<int64_t>(span / 512, 1);  // a part is worth a launch's join from 512 positions on
-    want = std::max<int64_t>(1, std::min<int64_t>({want, most, 64}));
-    k.most = (int)want;
+    auto parts = [&](int64_t span) -> int64_t {
+        if (k.chunk) return chunk_parts(units, span, (int64_t)c.nrows * heads, hd);
+        // two CTAs an SM; a part is worth its join from 512 positions on
+        int64_t want = std::max<int64_t>(1, std::min<int64_t>({(2 * 148 + units - 1) / units, span / 512, 64}));
+        // a warp sums every 8th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
+        // float32 results are joined from parts of at most 4096 positions
+        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 4095) / 4096);
+        return want;
+    };
+    const int64_t span = span_of(window);
+    const int64_t want = parts(span);
     k.part = (int)((span + want - 1) / want + 127) / 128 * 128;
-    k.splits = (int)((span + k.part - 1) / k.part);
-    if (k.splits < 1) k.splits = 1;
+    k.splits = std::max((int)((span + k.part - 1) / k.part), 1);
     return k;
+}
+
+// The most parts that any window gives: what the workspace has room for.
+int64_t most_parts(const Kv8 &c, int heads, int hd, int type) {
+    const Cut k = attention_cut(c, heads, hd, type, 0);
+    if (k.chunk) return std::min<int64_t>(64, (c.cap + 127) / 128);
+    const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
+    return std::max<int64_t>({1, std::min<int64_t>({(2 * 148 + units - 1) / units, c.cap / 512, 64}), type == LLMB_F32 ? ((int64_t)c.cap + 4095) / 4096 : 1});
 }
 
 }  // namespace
@@ -680,8 +715,8 @@ int64_t llmb_kv8_attention_workspace(const llmb_kv8_cache *cache, const llmb_kv8
         op_error(LLMB_ERR_ARG, "llm: kv8_attention_workspace: %d heads on %d kv heads", heads, c.kvh);
         return -1;
     }
-    int splits = 1;
-    for (int tile : {8, 16}) splits = std::max(splits, attention_cut(c, heads, tile, 0).most);
+    int64_t splits = 1;
+    for (int type : {LLMB_F32, LLMB_BF16}) splits = std::max(splits, most_parts(c, heads, cache->head_dim, type));
     return splits == 1 ? 0 : (int64_t)c.nrows * heads * splits * (8 + 4 * (int64_t)cache->head_dim);
 }
 
@@ -703,7 +738,7 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
     if ((rc = kv8_pointers(what, &dev, c, q, "q", out, "out", c.nrows == 0)) != LLMB_OK) return rc;
     if (c.max_new == 0) return LLMB_OK;
     Kv8Att a{};
-    const Cut cut = attention_cut(c, heads, type == LLMB_BF16 ? 16 : 8, window);
+    const Cut cut = attention_cut(c, heads, hd, type, window);
     if ((int64_t)c.kvh * cut.tiles > 65535)
         return op_error(LLMB_ERR_ARG, "llm: %s: %d rows of a sequence are too many", what, c.max_new);
     const int64_t slots = (int64_t)c.nrows * heads * cut.splits;
@@ -721,12 +756,19 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
     a.scale = (float)((scale != 0.f ? (double)scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
     a.tile = cut.tile, a.splits = cut.splits, a.part = cut.part;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    by_type(type, [&](auto t) {
+    const dim3 grid(cut.splits, c.kvh * cut.tiles, c.nseq);
+    if (cut.chunk) {
+        const cudaError_t e = kv8_chunk_launch(type, cache->type == LLMB_KV8_E4M3, hd, c, a, grid, st);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return op_error(LLMB_ERR_CUDA, "llm: %s: %s", what, cudaGetErrorString(e));
+        }
+    } else by_type(type, [&](auto t) {
         by_cache(cache->type, hd, [&](auto e4m3, auto d) {
             using T = decltype(t);
             constexpr int HD = decltype(d)::value;
             k_kv8_attend<T, decltype(e4m3)::value, HD, kPieces<T>>
-                <<<dim3(cut.splits, c.kvh * cut.tiles, c.nseq), kAttWarps * 32, 0, st>>>(c, a);
+                <<<grid, kAttWarps * 32, 0, st>>>(c, a);
         });
     });
     if ((rc = op_launched(what)) != LLMB_OK || cut.splits == 1) return rc;

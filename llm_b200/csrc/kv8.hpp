@@ -102,6 +102,16 @@ __device__ __forceinline__ float kv8_exp2(float x) {
     return r;
 }
 
+// The power of two that brings a query row whose largest magnitude has the bits m to [2^14, 2^15) (rows below 2^-100 by
+// the factor of 2^-100), and its inverse; false where the row is not finite (up is 0 then).
+__device__ __forceinline__ bool kv8_query_scale(uint32_t m, float &up, float &down) {
+    const bool fine = m < 0x7f800000u;
+    const int ex = m == 0 ? 0 : max((int)(m >> 23) - 127, -100);
+    up = fine ? __uint_as_float((uint32_t)(127 + 14 - ex) << 23) : 0.f;
+    down = __uint_as_float((uint32_t)(127 - 14 + (fine ? ex : 0)) << 23);
+    return fine;
+}
+
 constexpr int kKv8MaxGroup = 64;  // query heads of one kv head
 
 // ---- the attention's split of positions, as both its kernels see it
