@@ -10,13 +10,18 @@
 //           x = x + bias(v)
 //   mask:   x = -inf where v's bit is 0
 //
-// One pass over the vocabulary: the CTAs of a cluster share a row and hold a
-// slice of it in registers.  While those loads are under way each CTA counts
-// the history's tokens of its slice in a table in shared memory, a 32-bit
-// word per token id: the count in bits 13..31, bit 12 for the prompt's tokens,
-// in bits 0..11 the place of the token's bias (1..4095).  Counts are integers
-// and of a token's biases the last counts, so the order of the atomics does
-// not matter.  The cluster's first CTA takes the largest of the slices' maxima.
+// One pass over the vocabulary: the CTAs of a cluster share a row; chunks of
+// 32 tokens go round among them, so that the frequent tokens, which have low
+// ids, do not all fall to one.  A CTA counts the history's tokens among its
+// own in a table in shared memory, a 32-bit word per token: the count in bits
+// 13..31, bit 12 for the prompt's tokens, in bits 0..11 the place of the
+// token's bias (1..4095).  Counts are integers and of a token's biases the
+// last counts, so the order of the atomics does not matter.  Whoever touches a
+// word first lists it; then each listed token's logit is worked out, left in
+// its word, and marked in a bitmap.  The pass over the logits has only the
+// bits to look at (working tokens out there cost 57 instructions a logit: a
+// warp meets one of the history in most of its 128).  The cluster's first CTA
+// takes the largest of the CTAs' maxima; the others do not wait for it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -35,7 +40,7 @@ namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 512;
-constexpr int kMaxSlice = 11264;  // table words of a CTA: 44 KiB, so that four CTAs fit an SM
+constexpr int kMaxSlice = 11264;  // tokens of a CTA and round: 68 KiB with bitmap and list, three CTAs an SM
 constexpr int kMaxBias = 4095, kMaxHistory = (1 << 19) - 1;
 
 struct Ctl {
@@ -59,17 +64,26 @@ __device__ __forceinline__ uint64_t rank_of(float x, int v) {
     return (uint64_t)key << 32 | (uint32_t)~v;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t su32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_logits(const Ctl c) {
-    constexpr int E = 16 / (int)sizeof(T), NV = (kMaxSlice / E + kThreads - 1) / kThreads;
-    extern __shared__ uint32_t table[];
-    __shared__ uint64_t best_w[kThreads / 32], best_c[16];
+__global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
+    constexpr int E = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) uint32_t table[];  // c.slice words (a multiple of 32), their bitmap, the list
+    uint32_t *done = table + c.slice;
+    uint16_t *list = reinterpret_cast<uint16_t *>(done + c.slice / 32);
+    __shared__ uint64_t best_w[kThreads / 32], best_c[16], bar;
+    __shared__ int listed;
     cg::cluster_group cluster = cg::this_cluster();
-    if (c.tokens) cluster_arrive();  // waited for before the first access to another CTA's shared memory
-    const int nc = gridDim.x, rank = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+    const int nc = gridDim.x, rank = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    const int shift = 31 - __clz(nc);  // (a power of two)
+    if (c.tokens) {  // the first CTA's barrier counts the others' maxima; they may come once the cluster has started
+        if (tid == 0) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(&bar)), "r"(nc));
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
     const T *in = static_cast<const T *>(c.logits) + (int64_t)row * c.stride;
     T *out = c.out ? static_cast<T *>(c.out) + (int64_t)row * c.out_stride : nullptr;
     const uint32_t *mask = c.mask ? c.mask + (int64_t)row * c.mask_stride : nullptr;
@@ -84,104 +98,165 @@ __global__ void __launch_bounds__(kThreads) k_logits(const Ctl c) {
         bias0 = min(max(__ldg(c.bias_starts + row), 0), c.n_bias);
         bias1 = min(min(max(__ldg(c.bias_starts + row + 1), bias0), c.n_bias), bias0 + kMaxBias);
     }
-    uint64_t best = 0;
+    float best_x = -INFINITY;
+    int best_v = 0;
     for (int round = 0; round < c.rounds; ++round) {
-        const int64_t first = (int64_t)(round * nc + rank) * c.slice;
-        if (first >= c.vocab) break;
-        const int v0 = (int)first, n = min(c.slice, c.vocab - v0);
-        // the slice's logits, all on their way before the table is made
-        uint4 raw[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int u = (tid + i * kThreads) * E;
-            if (u >= n) continue;
-            if (VEC && u + E <= n) {
-                raw[i] = *reinterpret_cast<const uint4 *>(in + v0 + u);
+        const int chunk0 = round * (c.slice / 32);  // this round's first chunk of the CTA's
+        // the CTA's token u of the round, and back (-1: another's)
+        auto token = [&](int u) { return (((chunk0 + (u >> 5)) << shift) + rank) * 32 + (u & 31); };
+        auto place = [&](int v) {
+            if (v < 0 || v >= c.vocab || ((v >> 5) & (nc - 1)) != rank) return -1;
+            const int j = (v >> (5 + shift)) - chunk0;
+            return j >= 0 && j < c.slice / 32 ? j * 32 + (v & 31) : -1;
+        };
+        auto load = [&](int u, uint4 &raw) {
+            const int v = token(u);
+            if (VEC && v + E <= c.vocab) {
+                raw = *reinterpret_cast<const uint4 *>(in + v);
             } else {
                 T e[E];
 #pragma unroll
-                for (int k = 0; k < E; ++k) e[k] = u + k < n ? in[v0 + u + k] : kv8_from<T>(0.f);
-                raw[i] = *reinterpret_cast<const uint4 *>(e);
+                for (int k = 0; k < E; ++k) e[k] = v + k < c.vocab ? in[v + k] : kv8_from<T>(0.f);
+                raw = *reinterpret_cast<const uint4 *>(e);
             }
-        }
+        };
+        constexpr int step = kThreads * E;
+        // the first two vectors of the thread are on their way while the table is made
+        uint4 r0, r1;
+        if (tid * E < c.slice) load(tid * E, r0);
+        if (tid * E + step < c.slice) load(tid * E + step, r1);
         if (round > 0) __syncthreads();
-        for (int i = tid; i < n; i += kThreads) table[i] = 0;
+        if (nh > 0 || bias1 > bias0)
+            for (int i = 4 * tid; i < c.slice; i += 4 * kThreads) *reinterpret_cast<uint4 *>(table + i) = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < c.slice / 32; i += kThreads) done[i] = 0;
+        if (tid == 0) listed = 0;
         __syncthreads();
+        // (whole warps go round, for the ballot)
+        auto enlist = [&](bool fresh, int off) {
+            const uint32_t m = __ballot_sync(kFull, fresh);
+            if (!m) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&listed, __popc(m));
+            at = __shfl_sync(kFull, at, 0) + __popc(m & ((1u << lane) - 1));
+            if (fresh) list[at] = (uint16_t)off;
+        };
         if (bias1 > bias0) {
-            for (int i = bias0 + tid; i < bias1; i += kThreads) {
-                const uint32_t off = (uint32_t)(__ldg(c.bias_ids + i) - v0);
-                if (off < (uint32_t)n) atomicMax(table + off, (uint32_t)(i - bias0 + 1));
+            for (int i = bias0 + tid; i - lane < bias1; i += kThreads) {
+                const int off = i < bias1 ? place(__ldg(c.bias_ids + i)) : -1;
+                enlist(off >= 0 && atomicMax(table + off, (uint32_t)(i - bias0 + 1)) == 0, off);
             }
             __syncthreads();
         }
-        for (int i = tid; i < nh; i += kThreads) {
-            const uint32_t off = (uint32_t)(__ldg(hist + i) - v0);
-            if (off < (uint32_t)n) {
-                if (i < np) atomicOr(table + off, 1u << 12);
-                else atomicAdd(table + off, 1u << 13);
-            }
+#pragma unroll 2
+        for (int i = tid; i - lane < nh; i += kThreads) {
+            const int off = i < nh ? place(__ldg(hist + i)) : -1;
+            uint32_t old = 1;
+            if (off >= 0) old = i < np ? atomicOr(table + off, 1u << 12) : atomicAdd(table + off, 1u << 13);
+            enlist(old == 0, off);
         }
         __syncthreads();
+        for (int i = tid; i < listed; i += kThreads) {
+            const int off = list[i];
+            const uint32_t w = table[off];
+            float y = kv8_float<T>(in[token(off)]);
+            if (w >> 12) {
+                y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                if (w >> 13) y = __fsub_rn(__fsub_rn(y, pres), __fmul_rn(freq, (float)(w >> 13)));
+            }
+            if (w & 0xfffu) y = __fadd_rn(y, __ldg(c.bias_values + bias0 + (w & 0xfffu) - 1));
+            table[off] = __float_as_uint(y);
+            atomicOr(done + off / 32, 1u << (off % 32));
+        }
+        __syncthreads();
+        auto use = [&](int u, const uint4 &raw) {
+            const T *e = reinterpret_cast<const T *>(&raw);
+            const int v = token(u);
+            if (v >= c.vocab) return;
+            float x[E];
+            // E divides 32 and u is a multiple of E: one word of the mask and of the bitmap
+            uint32_t bits = mask ? __ldg(mask + (v >> 5)) >> (v & 31) : 0xffffffffu;
+            if (v + E > c.vocab) bits &= (1u << (c.vocab - v)) - 1;
+            const uint32_t fixed = done[u >> 5] >> (u & 31) & ((1u << E) - 1);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int u = (tid + i * kThreads) * E;
-            if (u >= n) continue;
-            const T *e = reinterpret_cast<const T *>(&raw[i]);
+            for (int k = 0; k < E; ++k) x[k] = kv8_float<T>(e[k]);
+            if (fixed) {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (fixed >> k & 1) x[k] = __uint_as_float(table[u + k]);
+            }
             T res[E];
-            // E divides 32 and v0 + u is a multiple of E: one mask word
-            const uint32_t bits = mask ? __ldg(mask + (v0 + u) / 32) >> ((v0 + u) % 32) : 0xffffffffu;
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                float x = kv8_float<T>(e[k]);
-                const uint32_t w = u + k < n ? table[u + k] : 0;
-                if (w >> 12) {
-                    x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-                    if (w >> 13) x = __fsub_rn(__fsub_rn(x, pres), __fmul_rn(freq, (float)(w >> 13)));
-                }
-                if (w & 0xfffu) x = __fadd_rn(x, __ldg(c.bias_values + bias0 + (w & 0xfffu) - 1));
-                if (!(bits >> k & 1)) x = -INFINITY;
-                res[k] = kv8_from<T>(x);
-                if (u + k < n) {
-                    const uint64_t r = rank_of(x, v0 + u + k);
-                    best = r > best ? r : best;
-                }
+                if (!(bits >> k & 1)) x[k] = -INFINITY;
+                res[k] = kv8_from<T>(x[k]);
+                if (x[k] > best_x) best_x = x[k], best_v = v + k;  // (the thread's tokens come in order)
             }
             if (out) {
-                if (VEC && u + E <= n) {
-                    *reinterpret_cast<uint4 *>(out + v0 + u) = *reinterpret_cast<const uint4 *>(res);
+                if (VEC && v + E <= c.vocab) {
+                    *reinterpret_cast<uint4 *>(out + v) = *reinterpret_cast<const uint4 *>(res);
                 } else {
 #pragma unroll
                     for (int k = 0; k < E; ++k)
-                        if (u + k < n) out[v0 + u + k] = res[k];
+                        if (v + k < c.vocab) out[v + k] = res[k];
                 }
             }
+        };
+        for (int u = tid * E; u < c.slice; u += 2 * step) {
+            const uint4 now = r0;
+            if (u + 2 * step < c.slice) load(u + 2 * step, r0);
+            use(u, now);
+            if (u + step >= c.slice) break;
+            const uint4 next = r1;
+            if (u + 3 * step < c.slice) load(u + 3 * step, r1);
+            use(u + step, next);
         }
     }
     if (!c.tokens) return;
+    uint64_t best = rank_of(best_x, best_v);
     for (int o = 16; o; o >>= 1) {
         const uint64_t r = __shfl_xor_sync(kFull, best, o);
         best = r > best ? r : best;
     }
-    if ((tid & 31) == 0) best_w[tid >> 5] = best;
-    cluster_wait();
+    if (lane == 0) best_w[tid >> 5] = best;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) best = best_w[w] > best ? best_w[w] : best;
-        *cluster.map_shared_rank(&best_c[rank], 0) = best;
+    if (tid < 32) {
+        best = tid < kThreads / 32 ? best_w[tid] : 0;
+        for (int o = 16; o; o >>= 1) {
+            const uint64_t r = __shfl_xor_sync(kFull, best, o);
+            best = r > best ? r : best;
+        }
     }
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-        for (int w = 0; w < nc; ++w) best = best_c[w] > best ? best_c[w] : best;
-        c.tokens[row] = best ? (int32_t)~(uint32_t)best : -1;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid != 0) return;
+    *cluster.map_shared_rank(&best_c[rank], 0) = best;
+    uint32_t first;  // the first CTA's barrier
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(su32(&bar)));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first) : "memory");
+    if (rank != 0) return;
+    bool ok = false;
+    for (int i = 0; i < 1 << 22 && !ok; ++i) {  // the others' work is a few microseconds; each try waits a while itself
+        uint32_t p;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(p)
+            : "r"(su32(&bar))
+            : "memory");
+        ok = p != 0;
     }
+    for (int w = 0; w < nc; ++w) best = best_c[w] > best ? best_c[w] : best;
+    c.tokens[row] = ok && best ? (int32_t)~(uint32_t)best : -1;
 }
 
-// Clusters of 16 CTAs are above the portable size; each kernel is told so once per device.
+constexpr size_t slice_bytes(int slice) { return (size_t)slice * 4 + slice / 8 + (size_t)slice * 2; }
+
+// Clusters of 16 CTAs are above the portable size and the table above the default's; each kernel is told so once per device.
 template <class T, bool VEC>
 cudaError_t allow_clusters(int device) noexcept {
     static std::atomic<bool> done[64];
     if (device < 64 && done[device].load(std::memory_order_relaxed)) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(k_logits<T, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(k_logits<T, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k_logits<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)slice_bytes(kMaxSlice));
     if (e == cudaSuccess && device < 64) done[device].store(true, std::memory_order_relaxed);
     return e;
 }
@@ -194,7 +269,7 @@ cudaError_t launch(const Ctl &c, int rows, int ctas, int device, cudaStream_t st
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(ctas, rows), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = (size_t)c.slice * 4;
+    cfg.gridDim = dim3(ctas, rows), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = slice_bytes(c.slice);
     cfg.stream = st, cfg.attrs = &attr, cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, k_logits<T, VEC>, c);
 }
@@ -240,9 +315,9 @@ extern "C" int llmb_logits_control(const void *logits, int64_t stride, int type,
     int ctas = 1;
     while (ctas < 16 && ctas * kThreads * 16 / es < vocab) ctas *= 2;
     Ctl c{};
-    c.rounds = (int)((vocab + (int64_t)ctas * kMaxSlice - 1) / ((int64_t)ctas * kMaxSlice));
-    c.slice = (vocab + ctas * c.rounds - 1) / (ctas * c.rounds);
-    c.slice = (c.slice + 127) / 128 * 128;
+    const int chunks = (vocab + 32 * ctas - 1) / (32 * ctas);  // of 32 tokens, for each CTA
+    c.rounds = (chunks + kMaxSlice / 32 - 1) / (kMaxSlice / 32);
+    c.slice = (chunks + c.rounds - 1) / c.rounds * 32;
     c.logits = logits, c.out = out, c.stride = stride, c.out_stride = out_stride, c.tokens = tokens;
     c.history = ctl->history, c.hist_lens = ctl->history_lens, c.prompt_lens = ctl->prompt_lens;
     c.hist_stride = ctl->history_stride, c.penalties = ctl->penalties;
