@@ -308,7 +308,7 @@ LLMB_API int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *ba
  * n_rows rows of [heads][head_dim] elements of `type`, q_stride and
  * out_stride elements apart, 16-byte aligned; out must not overlap q unless
  * it is the same buffer with the same stride.  scale 0 means
- * 1 / sqrt(head_dim).  A row that sees no position becomes 0, one whose query
+ * 1 / sqrt(head_dim), negative ones are refused.  A row that sees no position becomes 0, one whose query
  * is not finite NaN; rows of no sequence stay as they were.  `workspace`:
  * llmb_kv8_attention_workspace bytes of the caller's, 16-byte aligned, not
  * read before it is written; calls that may overlap on the GPU need their

@@ -197,10 +197,17 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
 
 constexpr int kAttWarps = 8;
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+}
+
+// The 8 x 8 matrix of 16-bit values whose row `lane / 4`, columns 2 (lane % 4) .. + 1 this lane holds, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -208,37 +215,74 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Attention of a tile of rows of one (sequence, kv head) over one part of the
+// The four 8-bit values of w as two pairs of float16, exactly (bytes 0 and 1, bytes 2 and 3).
+template <bool E4M3>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (E4M3) {
+        asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    } else {  // u = q + 128 under 1024's exponent is 1024 + u
+        const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 k = __half2half2(__float2half_rn(1152.f));
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), k), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), k);
+        lo = *reinterpret_cast<const uint32_t *>(&x), hi = *reinterpret_cast<const uint32_t *>(&y);
+    }
+}
+
+// What 16 positions share: where they lie in the pools (below 0: nowhere), K's scale, V's scale = mv 2^lv with 2^-lv.
+struct Place {
+    int64_t at;
+    float ks, lv, mv, unlv;
+};
+
+// Attention of 8 NB rows of one (sequence, kv head) over one part of the
 // positions: softmax with a running maximum, both products as m16n8k16 with
-// the 8-bit values exact in float16.
+// the 8-bit values exact in float16.  The cache is the left operand of both
+// (S^T = K Q^T, O^T = V^T P^T), so the few rows fill the 8 columns and each
+// value of the cache is converted once.
 //
-// A warp takes every 8th group of 16 positions, straight from global memory
-// into its registers: the contraction's index may be permuted as long as both
-// operands agree, so lane (g, t) = (lane / 4, lane % 4) loads 16 contiguous
-// bytes of K row g and uses them as its B fragments, and HD / 8 contiguous
-// bytes of the V rows 2t, 2t + 1, 2t + 8, 2t + 9.
+// A warp takes every 8th group of 16 positions, the next ones on their way
+// (asynchronous copies) while one is worked on.  The contraction's index may
+// be permuted as long as both operands agree, so lane (g, t) = (lane / 4,
+// lane % 4) copies 16 contiguous bytes of the K rows g and g + 8 and uses them
+// as its A fragments, and HD / 8 contiguous bytes of the V rows 2t, 2t + 1,
+// 2t + 8, 2t + 9, whose bytes j, paired by two rows, are A fragments of
+// elements g HD / 8 + j: each lane reads back only what it copied itself.  P
+// comes out as accumulators of S^T and is transposed 8 x 8 into B fragments.
+// A lane looks up the place of one group in 32 ahead of time.
 //
 // float32 rows (PIECES = 2) are the sum of two float16 pieces, which hold 22
 // bits of the row's largest element after a power of two has brought it to
-// [2^14, 2^15): the upper 8 rows of a matrix tile are the first pieces, the
-// lower 8 the second, and lane (g, t) holds both results.  The weights go
-// into the second product the same way.  bfloat16 rows fill a tile of 16.
+// [2^14, 2^15); the weights go into the second product the same way.
+// float16 rows fit one piece, but a weight rounded to float16 is off as much
+// as the result's own rounding, so they take the two-piece form as well.
 //
 // The scale of V's block enters the weights' exponent (its power of two, so
 // that the largest weight of all stays near 2^6 and float16 holds the small
 // ones) and mantissa.
-//
-// float16 rows fit one piece, but a weight rounded to float16 is off as much
-// as the result's own rounding, so they take the two-piece form as well.
 template <class T>
 constexpr int kPieces = 2;
 template <>
 constexpr int kPieces<__nv_bfloat16> = 1;
 
-template <class T, bool E4M3, int HD, int PIECES>
-__global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, const Kv8Att a) {
-    constexpr int ROWS = PIECES == 2 ? 8 : 16, NR = PIECES == 2 ? 1 : 2;  // rows of a tile; of a lane
-    constexpr int KS = HD / 16, NT = HD / 8;                              // k steps; column tiles of V
+// Groups of a warp in flight, as many as two CTAs an SM have room for (a group is 32 HD bytes), and their bytes.
+__host__ __device__ constexpr int att_depth(int hd) { return hd == 64 ? 5 : 3; }
+__host__ __device__ constexpr int att_smem(int hd) { return kAttWarps * att_depth(hd) * 32 * hd; }
+
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <class T, bool E4M3, int HD, int NB>
+__global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(const Kv8 c, const Kv8Att a) {
+    constexpr int PIECES = kPieces<T>, ROWS = 8 * NB, KS = HD / 16, NT = HD / 16;  // k steps; tiles of 16 elements of V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int s = blockIdx.z, head = blockIdx.y % c.kvh, row0 = blockIdx.y / c.kvh * ROWS;
     const Kv8Seq sq = kv8_seq(c, s);
@@ -251,20 +295,82 @@ __global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, cons
     if (blockIdx.x > 0 && lo + (int64_t)blockIdx.x * a.part >= hi) return;
     lo += blockIdx.x * a.part;
     hi = min(hi, lo + a.part);
+    // every row sees all of [all0, all1)
+    const int all0 = a.window > 0 ? max(sq.first + tok1 + 1 - a.window, lo) : lo, all1 = min(sq.first + tok0 + 1, hi);
 
-    // the rows' queries as A fragments
-    uint32_t qf[KS][4];
-    float fac[NR];
-    int pos[NR];
+    constexpr int step = 16 * kAttWarps;
+    auto look_up = [&](int p) {
+        Place x = {-1, 0.f, 0.f, 0.f, 0.f};
+        const int b = p < hi ? kv8_block(c, s, p >> c.bshift) : -1;
+        if (b < 0) return x;
+        x.at = b * c.bstride + ((int64_t)head * c.block + (p & (c.block - 1))) * HD;
+        x.ks = __ldg(c.ks + (int64_t)b * c.kvh + head);
+        const float vs = __ldg(c.vs + (int64_t)b * c.kvh + head);
+        const bool normal = vs >= FLT_MIN && vs <= FLT_MAX;  // (smaller ones, 0 among them, are factors as they are)
+        const uint32_t u = __float_as_uint(vs);
+        const int ex = normal ? (int)(u >> 23) - 127 : 0;
+        x.lv = (float)ex, x.mv = normal ? __uint_as_float((u & 0x7fffffu) | 0x3f800000u) : vs;
+        x.unlv = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
+        return x;
+    };
+    auto of_lane = [&](const Place &x, int i) {
+        Place y;
+        y.at = __shfl_sync(kFull, x.at, i);
+        y.ks = __shfl_sync(kFull, x.ks, i), y.lv = __shfl_sync(kFull, x.lv, i);
+        y.mv = __shfl_sync(kFull, x.mv, i), y.unlv = __shfl_sync(kFull, x.unlv, i);
+        return y;
+    };
+    // a group of 16 positions as a lane holds it
+    struct Group {
+        uint4 k[2][HD / 64];
+        uint32_t v[4][HD / 32];
+        Place at;
+    };
+    const int k_lane = g * HD + 16 * t, v_lane = 2 * t * HD + g * (HD / 8);
+    extern __shared__ __align__(16) uint8_t ring[];  // [warp][depth]: K's pieces [2][HD / 64][lane] of 16 bytes, V's [4][lane] of HD / 8
+    constexpr int D = att_depth(HD), VB = HD / 8;
+    uint8_t *mine = ring + warp * D * 32 * HD;
+    int p = lo + 16 * warp, copied = 0;  // groups of the warp whose copies were started
+    Place ahead = {-1, 0.f, 0.f, 0.f, 0.f};
+    // starts the copies of the warp's next group, if there is one, and closes their set
+    auto copy = [&]() {
+        const int p1 = p + copied * step;
+        if (p1 < hi) {
+            if (copied % 32 == 0) ahead = look_up(p1 + lane * step);
+            const int64_t at = __shfl_sync(kFull, ahead.at, copied % 32);
+            if (at >= 0) {
+                const uint8_t *kp = c.k + at + k_lane, *vp = c.v + at + v_lane;
+                uint8_t *dst = mine + copied % D * 32 * HD;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const int r = row0 + g + 8 * i;
-        const bool on = r < rows;
-        const int tok = r / a.group, h = head * a.group + r - tok * a.group;
-        pos[i] = on ? sq.first + tok : -1;
-        const T *qp = static_cast<const T *>(a.q) + (int64_t)(sq.start + (on ? tok : tok0)) * a.q_stride + (on ? h : head * a.group) * HD;
-        float x[KS][4], m = 0.f;
-        bool fine = true;
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < HD / 64; ++i) cp16(dst + ((n * (HD / 64) + i) * 32 + lane) * 16, kp + 8 * n * HD + 64 * i);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    uint8_t *to = dst + 16 * HD + (n * 32 + lane) * VB;
+                    const uint8_t *from = vp + ((n & 1) + 8 * (n >> 1)) * HD;
+                    if constexpr (HD == 64) cp8(to, from);
+                    else cp16(to, from);
+                }
+            }
+            ++copied;
+        }
+        cp_commit();
+    };
+    // the first groups are on their way before the queries are read
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) copy();
+
+    // the rows' queries as B fragments: row g of each 8
+    uint32_t qf[NB][PIECES][KS][2];
+    float fac[NB][2];   // rows 2t and 2t + 1, as the accumulators have them
+    int pos[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int r = min(row0 + 8 * i + g, last), tok = r / a.group, h = head * a.group + r - tok * a.group;
+        const T *qp = static_cast<const T *>(a.q) + (int64_t)(sq.start + tok) * a.q_stride + h * HD;
+        float x[KS][4];
+        uint32_t m = 0;  // the largest magnitude's bits; infinity and NaN are above the finite ones
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             // 16 bytes of K hold the 4 values of 4 steps: value e of step ks is element 64 (ks / 4) + 16 t + 4 (ks % 4) + e
@@ -273,192 +379,204 @@ __global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, cons
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(e);
             else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(e);
 #pragma unroll
-            for (int e2 = 0; e2 < 4; ++e2) {
-                x[ks][e2] = kv8_float<T>(v[e2]);
-                fine = fine && fabsf(x[ks][e2]) <= FLT_MAX;
-                m = fmaxf(m, fabsf(x[ks][e2]));
-            }
+            for (int e2 = 0; e2 < 4; ++e2) x[ks][e2] = kv8_float<T>(v[e2]), m = max(m, __float_as_uint(x[ks][e2]) & 0x7fffffffu);
         }
-        m = fmaxf(m, __shfl_xor_sync(kFull, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(kFull, m, 2));
-        fine = __shfl_xor_sync(kFull, (int)fine, 1) && fine;
-        fine = __shfl_xor_sync(kFull, (int)fine, 2) && fine;
-        // m = [1, 2) 2^e becomes [2^14, 2^15); a row that is not finite has NaN as its factor
-        const int ex = fine && m > 0.f ? max(ilogbf(m), -100) : 0;
-        const float up = fine ? scalbnf(1.f, 14 - ex) : 0.f;
-        fac[i] = fine ? a.scale * kv8_unit<E4M3>() * scalbnf(1.f, ex - 14) : NAN;
+        m = max(m, __shfl_xor_sync(kFull, m, 1));
+        m = max(m, __shfl_xor_sync(kFull, m, 2));
+        float up, down;
+        const bool fine = kv8_query_scale(m, up, down);
+        const float f = fine ? a.scale * down : NAN;  // a row that is not finite has NaN as its factor
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = fine ? x[ks][e] * up : 0.f;
-            const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
-            qf[ks][i] = h0, qf[ks][2 + i] = h1;
-            if (PIECES == 2) {
-                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
-                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
-                qf[ks][1] = pack_half2(y[0] - f0.x, y[1] - f0.y);
-                qf[ks][3] = pack_half2(y[2] - f1.x, y[3] - f1.y);
-            }
-        }
-    }
-
-    float o[NT][4], m[NR], l[NR];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) m[i] = -FLT_MAX, l[i] = 0.f;
-
-    // a group of 16 positions as a lane holds it
-    struct Group {
-        uint4 k[2][HD / 64];
-        uint32_t v[4][HD / 32];
-        float ks, vs;
-        int b;
-    };
-    auto load = [&](Group &x, int p0) {
-        if (p0 >= hi) {
-            x.b = -1;
-            return;
-        }
-        x.b = kv8_block(c, s, p0 >> c.bshift);
-        if (x.b < 0) return;
-        const int64_t at = x.b * c.bstride + ((int64_t)head * c.block + (p0 & (c.block - 1))) * HD;
-        const uint8_t *kp = c.k + at, *vp = c.v + at;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < HD / 64; ++i)
-                x.k[n][i] = __ldg(reinterpret_cast<const uint4 *>(kp + (8 * n + g) * HD + 64 * i + 16 * t));
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const uint8_t *r = vp + (2 * t + (n & 1) + 8 * (n >> 1)) * HD + g * (HD / 8);
-            if constexpr (HD == 64) {
-                const uint2 w = __ldg(reinterpret_cast<const uint2 *>(r));
-                x.v[n][0] = w.x, x.v[n][1] = w.y;
-            } else {
-                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(r));
-                x.v[n][0] = w.x, x.v[n][1] = w.y, x.v[n][2] = w.z, x.v[n][3] = w.w;
-            }
-        }
-        x.ks = __ldg(c.ks + (int64_t)x.b * c.kvh + head);
-        x.vs = __ldg(c.vs + (int64_t)x.b * c.kvh + head);
-    };
-    auto use = [&](const Group &x, int p0) {
-        if (x.b < 0) return;
-        float sc[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint4 &w4 = x.k[n][ks / 4];
-                const uint32_t w = ks % 4 == 0 ? w4.x : ks % 4 == 1 ? w4.y : ks % 4 == 2 ? w4.z : w4.w;
-                mma16816(sc[n], qf[ks], kv8_half2<E4M3>(__byte_perm(w, 0, 0x4140)),
-                         kv8_half2<E4M3>(__byte_perm(w, 0, 0x4342)));
-            }
-        }
-        // V's scale = mv 2^lv
-        const bool has = x.vs > 0.f;
-        const int lv = has ? ilogbf(x.vs) : 0;
-        const float mv = has ? scalbnf(x.vs, -lv) : x.vs, flv = (float)lv, unlv = scalbnf(1.f, -lv);
-        float z[NR][4];  // scores in log2, V's exponent added; position 16 + 8 (e / 2) + 2 t + e % 2
-        bool up = false;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const float f = fac[i] * x.ks;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float d = PIECES == 2 ? sc[e >> 1][e & 1] + sc[e >> 1][2 + (e & 1)] : sc[e >> 1][2 * i + (e & 1)];
-                const int p = p0 + 8 * (e >> 1) + 2 * t + (e & 1);
-                const bool seen = p <= pos[i] && p < hi && (a.window == 0 || p > pos[i] - a.window);
-                z[i][e] = seen ? fmaf(d, f, flv) : -INFINITY;
-                up |= z[i][e] - m[i] > 8.f;
-            }
-        }
-        if (__any_sync(kFull, up)) {
-#pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                float n = fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3]));
-                n = fmaxf(n, __shfl_xor_sync(kFull, n, 1));
-                n = fmaxf(n, __shfl_xor_sync(kFull, n, 2));
-                n = fmaxf(n, m[i]);
-                const float r = kv8_exp2(m[i] - n);
-                m[i] = n;
-                l[i] *= r;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    o[j][2 * i] *= r, o[j][2 * i + 1] *= r;
-                    if (PIECES == 2) o[j][2] *= r, o[j][3] *= r;
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t w = pack_half2(y[2 * j], y[2 * j + 1]);
+                qf[i][0][ks][j] = w;
+                if constexpr (PIECES == 2) {
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                    qf[i][1][ks][j] = pack_half2(y[2 * j] - b.x, y[2 * j + 1] - b.y);
                 }
             }
         }
-        uint32_t pf[4];
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            float w[4], sum = 0.f;
+        for (int e = 0; e < 2; ++e) {
+            fac[i][e] = __shfl_sync(kFull, f, 4 * (2 * t + e));
+            const int r2 = row0 + 8 * i + 2 * t + e;
+            pos[i][e] = r2 <= last ? sq.first + r2 / a.group : -1;
+        }
+    }
+
+    float o[NB][NT][4], m[NB][2], l[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+        m[i][0] = m[i][1] = -FLT_MAX, l[i][0] = l[i][1] = 0.f;
+    }
+
+    auto use = [&](Group &x, int p0) {
+        const bool whole = p0 >= all0 && p0 + 16 <= all1;
+        float sc[NB][4];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint32_t k0[2], k1[2];
+            auto word = [&](const uint4 &w) { return ks % 4 == 0 ? w.x : ks % 4 == 1 ? w.y : ks % 4 == 2 ? w.z : w.w; };
+            halves<E4M3>(word(x.k[0][ks / 4]), k0[0], k1[0]);
+            halves<E4M3>(word(x.k[1][ks / 4]), k0[1], k1[1]);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int q = PIECES - 1; q >= 0; --q) mma16816(sc[i], k0[0], k0[1], k1[0], k1[1], qf[i][q][ks]);
+        }
+        // sc[e]: position p0 + g + 8 (e / 2), row 2t + e % 2
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int q = p0 + g + 8 * (e >> 1);
+                    const bool seen = q <= pos[i][e & 1] && q < hi && (a.window == 0 || q > pos[i][e & 1] - a.window);
+                    if (!seen) sc[i][e] = -INFINITY;
+                }
+            // a byte behind the sequence's end may be a NaN of e4m3, which a weight of 0 would not stop
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (p0 + 2 * t + (n & 1) + 8 * (n >> 1) >= hi)
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) x.v[n][j] = 0;
+        }
+        float f[NB][2];
+        bool up = false;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                f[i][e] = fac[i][e] * x.at.ks;
+                const float top = fmaxf(sc[i][e], sc[i][2 + e]);
+                // scores in log2, V's exponent added (a position not seen and a factor 0: -inf * 0 is NaN, not above)
+                up |= fmaf(top, f[i][e], x.at.lv) - m[i][e] > 8.f;
+            }
+        if (__any_sync(kFull, up)) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                float r[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float top = fmaxf(sc[i][e], sc[i][2 + e]);
+                    float n = top > -INFINITY ? fmaf(top, f[i][e], x.at.lv) : -FLT_MAX;
+                    n = fmaxf(n, __shfl_xor_sync(kFull, n, 4));
+                    n = fmaxf(n, __shfl_xor_sync(kFull, n, 8));
+                    n = fmaxf(n, __shfl_xor_sync(kFull, n, 16));
+                    n = fmaxf(n, m[i][e]);
+                    r[e] = kv8_exp2(m[i][e] - n);
+                    m[i][e] = n;
+                    l[i][e] *= r[e];
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) o[i][j][0] *= r[0], o[i][j][1] *= r[1], o[i][j][2] *= r[0], o[i][j][3] *= r[1];
+            }
+        }
+        uint32_t pf[NB][PIECES][2];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                w[e] = kv8_exp2(z[i][e] - m[i] + 6.f);
-                sum += w[e];
-                w[e] *= mv;
+                w[e] = kv8_exp2(fmaf(sc[i][e], f[i][e & 1], x.at.lv + 6.f - m[i][e & 1]));
+                if (!whole && sc[i][e] == -INFINITY) w[e] = 0.f;
             }
-            l[i] = fmaf(sum, unlv, l[i]);
-            pf[i] = pack_half2(w[0], w[1]), pf[2 + i] = pack_half2(w[2], w[3]);
-            if (PIECES == 2) {
-                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&pf[0]));
-                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&pf[2]));
-                pf[1] = pack_half2(w[0] - f0.x, w[1] - f0.y);
-                pf[3] = pack_half2(w[2] - f1.x, w[3] - f1.y);
+            l[i][0] = fmaf(w[0] + w[2], x.at.unlv, l[i][0]), l[i][1] = fmaf(w[1] + w[3], x.at.unlv, l[i][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float w0 = w[2 * h] * x.at.mv, w1 = w[2 * h + 1] * x.at.mv;
+                const uint32_t y = pack_half2(w0, w1);
+                pf[i][0][h] = transpose8(y);
+                if constexpr (PIECES == 2) {
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+                    pf[i][1][h] = transpose8(pack_half2(w0 - b.x, w1 - b.y));
+                }
             }
         }
 #pragma unroll
-        for (int j = 0; j < NT; j += 4) {
-            // column tiles j .. j + 3 are the 4 bytes of word j / 4 of each V row
-            const uint32_t a0 = __byte_perm(x.v[0][j / 4], x.v[1][j / 4], 0x5140), a1 = __byte_perm(x.v[0][j / 4], x.v[1][j / 4], 0x7362);
-            const uint32_t b0 = __byte_perm(x.v[2][j / 4], x.v[3][j / 4], 0x5140), b1 = __byte_perm(x.v[2][j / 4], x.v[3][j / 4], 0x7362);
+        for (int j = 0; j < NT; j += 2) {
+            // tiles j and j + 1 are the bytes 0, 1 and 2, 3 of word j / 2 of each V row
+            const uint32_t v0 = x.v[0][j / 2], v1 = x.v[1][j / 2], v2 = x.v[2][j / 2], v3 = x.v[3][j / 2];
+            uint32_t a0[2], a1[2], b0[2], b1[2];
+            halves<E4M3>(__byte_perm(v0, v1, 0x5140), a0[0], a0[1]);  // byte 0 and byte 1 of rows 2t, 2t + 1
+            halves<E4M3>(__byte_perm(v0, v1, 0x7362), a1[0], a1[1]);
+            halves<E4M3>(__byte_perm(v2, v3, 0x5140), b0[0], b0[1]);
+            halves<E4M3>(__byte_perm(v2, v3, 0x7362), b1[0], b1[1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t sel = e & 1 ? 0x4342 : 0x4140;
-                mma16816(o[j + e], pf, kv8_half2<E4M3>(__byte_perm(e < 2 ? a0 : a1, 0, sel)),
-                         kv8_half2<E4M3>(__byte_perm(e < 2 ? b0 : b1, 0, sel)));
-            }
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int q = PIECES - 1; q >= 0; --q) {
+                    mma16816(o[i][j], a0[0], a0[1], b0[0], b0[1], pf[i][q]);
+                    mma16816(o[i][j + 1], a1[0], a1[1], b1[0], b1[1], pf[i][q]);
+                }
         }
     };
 
-    Group x0, x1;
-    const int step = 16 * kAttWarps;
-    int p = lo + 16 * warp;
-    load(x0, p);
-    for (; p < hi; p += 2 * step) {
-        load(x1, p + step);
-        use(x0, p);
-        load(x0, p + 2 * step);
-        use(x1, p + step);
+    // The places of the groups at hand; the copies, fewer than 32 groups ahead, may already be in the next set.
+    Place now = ahead;
+    int used = 0;
+    for (int q = p; q < hi; q += step, ++used) {
+        if (used % 32 == 0) now = ahead;
+        copy();  // (into the place of the group before this one)
+        cp_wait<D - 1>();
+        Group x;
+        x.at = of_lane(now, used % 32);
+        if (x.at.at < 0) continue;
+        const uint8_t *src = mine + used % D * 32 * HD;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) x.k[n][i] = *reinterpret_cast<const uint4 *>(src + ((n * (HD / 64) + i) * 32 + lane) * 16);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint8_t *from = src + 16 * HD + (n * 32 + lane) * VB;
+            if constexpr (HD == 64) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(from);
+                x.v[n][0] = w.x, x.v[n][1] = w.y;
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4 *>(from);
+                x.v[n][0] = w.x, x.v[n][1] = w.y, x.v[n][2] = w.z, x.v[n][3] = w.w;
+            }
+        }
+        use(x, q);
     }
 
     // the warps' results, joined 64 elements at a time
-    __shared__ float so[kAttWarps][ROWS][64 + 4];
+    static_assert(att_smem(HD) >= kAttWarps * ROWS * 68 * 4, "the results lie where the ring was");
+    float (*so)[ROWS][64 + 4] = reinterpret_cast<float (*)[ROWS][64 + 4]>(ring);
     __shared__ float2 sml[kAttWarps][ROWS];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        l[i] += __shfl_xor_sync(kFull, l[i], 1);
-        l[i] += __shfl_xor_sync(kFull, l[i], 2);
-        if (t == 0) sml[warp][g + 8 * i] = make_float2(m[i], l[i]);
-    }
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[i][e] += __shfl_xor_sync(kFull, l[i][e], 4);
+            l[i][e] += __shfl_xor_sync(kFull, l[i][e], 8);
+            l[i][e] += __shfl_xor_sync(kFull, l[i][e], 16);
+            if (g == 0) sml[warp][8 * i + 2 * t + e] = make_float2(m[i][e], l[i][e]);
+        }
     const int nrow = last - row0 + 1;
+    cp_wait<0>();
     for (int d0 = 0; d0 < HD; d0 += 64) {
-        if (d0 > 0) __syncthreads();
-        // column tile j's columns 2t, 2t + 1 are elements 2t HD/8 + j and (2t + 1) HD/8 + j
-        const int c0 = 2 * t * (HD / 8) - d0;
+        __syncthreads();
+        // o[j][e] is element g HD / 8 + 2 j + e / 2 of row 2t + e % 2
+        const int c0 = g * (HD / 8) - d0;
         if (c0 >= 0 && c0 < 64) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        so[warp][g + 8 * i][c0 + e * (HD / 8) + j] = PIECES == 2 ? o[j][e] + o[j][2 + e] : o[j][2 * i + e];
+                        *reinterpret_cast<float2 *>(&so[warp][8 * i + 2 * t + e][c0 + 2 * j]) = make_float2(o[i][j][e], o[i][j][2 + e]);
         }
         __syncthreads();
         for (int u = threadIdx.x; u < nrow * 64; u += kAttWarps * 32) {
@@ -472,7 +590,6 @@ __global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, cons
                 L = fmaf(f, sml[w][r].y, L);
                 O = fmaf(f, so[w][r][d], O);
             }
-            O *= kv8_unit<E4M3>();
             const int rr = row0 + r, tok = rr / a.group, h = head * a.group + rr - tok * a.group;
             if (a.splits == 1) {
                 // no position seen: every warp's sum is 0
@@ -487,37 +604,75 @@ __global__ void __launch_bounds__(kAttWarps * 32) k_kv8_attend(const Kv8 c, cons
     }
 }
 
-// Joins the parts of one (row, query head): a warp each.
-template <class T, int HD>
+// Joins the parts of one (row, query head): W warps of a block each.  Few rows have many parts (a single long sequence),
+// whose loads one warp would make one after the other: 37 parts 20 us with one warp, 3 us with eight.
+template <class T, int HD, int W>
 __global__ void __launch_bounds__(256) k_kv8_join(const Kv8 c, const Kv8Att a) {
+    constexpr int E = HD / 32;  // elements of a lane
     cudaGridDependencySynchronize();
-    const int lane = threadIdx.x & 31, s = blockIdx.z;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = blockIdx.z;
     const Kv8Seq sq = kv8_seq(c, s);
-    const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (r >= (int64_t)sq.n * a.heads) return;
-    const int tok = (int)(r / a.heads), h = (int)(r % a.heads), kvr = tok * a.group + h % a.group;
+    const int64_t r = (int64_t)blockIdx.x * (8 / W) + warp / W;
+    const bool on = r < (int64_t)sq.n * a.heads;
+    if (W == 1 && !on) return;
+    const int tok = on ? (int)(r / a.heads) : 0, h = on ? (int)(r % a.heads) : 0, kvr = tok * a.group + h % a.group;
     // the span of the row's tile, as its parts were cut
     const int row0 = kvr / a.tile * a.tile, last = min(row0 + a.tile, sq.n * a.group) - 1;
     int lo, hi;
     kv8_span(sq, a.window, row0 / a.group, last / a.group, lo, hi);
-    const int parts = max((hi - lo + a.part - 1) / a.part, 1);
+    const int parts = on ? max((hi - lo + a.part - 1) / a.part, 1) : 0;
     const int64_t at = ((int64_t)(sq.start + tok) * a.heads + h) * a.splits;
-    float M = -FLT_MAX;
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.part_ml[at + i].x);
-    for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, k));
-    float L = 0.f, O[HD / 32];
+    float M = -FLT_MAX, L = 0.f, O[E];
 #pragma unroll
-    for (int k = 0; k < HD / 32; ++k) O[k] = 0.f;
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = a.part_ml[at + i];
-        const float f = kv8_exp2(ml.x - M);
-        L = fmaf(f, ml.y, L);
+    for (int k = 0; k < E; ++k) O[k] = 0.f;
+    // the warp's parts are warp % W, + W, ...; a lane weighs one in 32
+    for (int i0 = warp % W; i0 < parts; i0 += 32 * W) {
+        const int mine = i0 + lane * W, n = min((parts - i0 + W - 1) / W, 32);
+        const float2 ml = mine < parts ? a.part_ml[at + mine] : make_float2(-FLT_MAX, 0.f);
+        float top = ml.x;
+        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
+        top = fmaxf(top, M);
+        const float old = kv8_exp2(M - top), f = kv8_exp2(ml.x - top);
+        M = top;
+        L = fmaf(L, old, f * ml.y);
 #pragma unroll
-        for (int k = 0; k < HD / 32; ++k) O[k] = fmaf(f, a.part_o[(at + i) * HD + lane + 32 * k], O[k]);
+        for (int k = 0; k < E; ++k) O[k] *= old;
+        const float *src = a.part_o + (at + i0) * HD + lane * E;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float w = __shfl_sync(kFull, f, i);
+            float v[E];
+            if constexpr (E == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(src + (int64_t)i * W * HD);
+            else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src + (int64_t)i * W * HD);
+#pragma unroll
+            for (int k = 0; k < E; ++k) O[k] = fmaf(w, v[k], O[k]);
+        }
     }
-    T *out = static_cast<T *>(a.out) + (int64_t)(sq.start + tok) * a.out_stride + h * HD;
+    for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(kFull, L, k);
+    if constexpr (W > 1) {
+        __shared__ float so[W][HD], sl[W], sm[W];
 #pragma unroll
-    for (int k = 0; k < HD / 32; ++k) out[lane + 32 * k] = kv8_from<T>(L == 0.f ? 0.f : O[k] / L);
+        for (int k = 0; k < E; ++k) so[warp][lane * E + k] = O[k];
+        if (lane == 0) sl[warp] = L, sm[warp] = M;
+        __syncthreads();
+        if (warp > 0 || !on) return;
+        for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w]);
+        L = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) O[k] = 0.f;
+        for (int w = 0; w < W; ++w) {
+            const float f = kv8_exp2(sm[w] - M);
+            L = fmaf(f, sl[w], L);
+#pragma unroll
+            for (int k = 0; k < E; ++k) O[k] = fmaf(f, so[w][lane * E + k], O[k]);
+        }
+    }
+    T v[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] = kv8_from<T>(L == 0.f ? 0.f : O[k] / L);
+    T *out = static_cast<T *>(a.out) + (int64_t)(sq.start + tok) * a.out_stride + h * HD + lane * E;
+#pragma unroll
+    for (int k = 0; k < E; ++k) out[k] = v[k];
 }
 
 // --------------------------------------------------------------- host --
@@ -541,7 +696,7 @@ int kv8_sizes(const char *what, const llmb_kv8_cache *c, const llmb_kv8_batch *b
         return op_error(LLMB_ERR_ARG, "llm: %s: %d sequences, %d table entries, %d rows, max_new %d, max_len %d", what,
                         b->n_seq, b->table_stride, b->n_rows, b->max_new, b->max_len);
     const int64_t held = (int64_t)b->table_stride * c->block;
-    if (held > INT32_MAX - 4096)
+    if (held > INT32_MAX - 16384)
         return op_error(LLMB_ERR_ARG, "llm: %s: tables of more than 2^31 positions", what);
     k = Kv8{};
     k.bstride = c->block_stride, k.nblocks = c->n_blocks, k.block = c->block, k.kvh = c->kv_heads;
@@ -600,6 +755,13 @@ void by_cache(int type, int hd, F &&f) {
     else hd == 64 ? f(No{}, std::integral_constant<int, 64>{}) : f(No{}, std::integral_constant<int, 128>{});
 }
 
+template <class T, bool E4M3, int HD, int NB>
+cudaError_t attend_launch(const Kv8 &c, const Kv8Att &a, dim3 grid, int device, cudaStream_t st) noexcept {
+    const cudaError_t e = op_shared<k_kv8_attend<T, E4M3, HD, NB>>(device, att_smem(HD));
+    if (e == cudaSuccess) k_kv8_attend<T, E4M3, HD, NB><<<grid, kAttWarps * 32, att_smem(HD), st>>>(c, a);
+    return e;
+}
+
 // How the attention cuts its work: rows into tiles, a tile's positions into parts.
 struct Cut {
     bool chunk;  // by the kernel for many rows
@@ -627,7 +789,7 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     const int64_t rows = (int64_t)c.max_new * group;
     // rows of one kv head from which on the tensor cores' tiles pay
     k.chunk = rows > 64;
-    const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 ? 16 : 8;
+    const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 && rows > 8 ? 16 : 8;
     k.tile = tile;
     k.tiles = (int)((rows + tile - 1) / tile);
     // the most positions that a tile's rows see between them
@@ -642,8 +804,8 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
         // two CTAs an SM; a part is worth its join from 512 positions on
         int64_t want = std::max<int64_t>(1, std::min<int64_t>({(2 * 148 + units - 1) / units, span / 512, 64}));
         // a warp sums every 8th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
-        // float32 results are joined from parts of at most 4096 positions
-        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 4095) / 4096);
+        // float32 results are joined from parts of at most 2048 positions
+        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 2047) / 2048);
         return want;
     };
     const int64_t span = span_of(window);
@@ -658,7 +820,7 @@ int64_t most_parts(const Kv8 &c, int heads, int hd, int type) {
     const Cut k = attention_cut(c, heads, hd, type, 0);
     if (k.chunk) return std::min<int64_t>(64, (c.cap + 127) / 128);
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
-    return std::max<int64_t>({1, std::min<int64_t>({(2 * 148 + units - 1) / units, c.cap / 512, 64}), type == LLMB_F32 ? ((int64_t)c.cap + 4095) / 4096 : 1});
+    return std::max<int64_t>({1, std::min<int64_t>({(2 * 148 + units - 1) / units, c.cap / 512, 64}), type == LLMB_F32 ? ((int64_t)c.cap + 2047) / 2048 : 1});
 }
 
 }  // namespace
@@ -730,7 +892,7 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
     const int hd = cache->head_dim;
     if (heads < 1 || heads % c.kvh != 0 || heads / c.kvh > kKv8MaxGroup)
         return op_error(LLMB_ERR_ARG, "llm: %s: %d heads on %d kv heads", what, heads, c.kvh);
-    if (window < 0 || !(std::fabs(scale) <= FLT_MAX))
+    if (window < 0 || !(scale >= 0.f && scale <= FLT_MAX))
         return op_error(LLMB_ERR_ARG, "llm: %s: window %d, scale %g", what, window, (double)scale);
     if ((rc = kv8_rows(what, type, q_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
     if ((rc = kv8_rows(what, type, out_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
@@ -757,32 +919,39 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
     a.tile = cut.tile, a.splits = cut.splits, a.part = cut.part;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid(cut.splits, c.kvh * cut.tiles, c.nseq);
-    if (cut.chunk) {
-        const cudaError_t e = kv8_chunk_launch(type, cache->type == LLMB_KV8_E4M3, hd, c, a, grid, st);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return op_error(LLMB_ERR_CUDA, "llm: %s: %s", what, cudaGetErrorString(e));
-        }
-    } else by_type(type, [&](auto t) {
+    cudaError_t e = cudaSuccess;
+    if (cut.chunk) e = kv8_chunk_launch(type, cache->type == LLMB_KV8_E4M3, hd, c, a, grid, dev, st);
+    else by_type(type, [&](auto t) {
         by_cache(cache->type, hd, [&](auto e4m3, auto d) {
             using T = decltype(t);
             constexpr int HD = decltype(d)::value;
-            k_kv8_attend<T, decltype(e4m3)::value, HD, kPieces<T>>
-                <<<grid, kAttWarps * 32, 0, st>>>(c, a);
+            constexpr bool E4 = decltype(e4m3)::value;
+            if constexpr (kPieces<T> == 1) {
+                if (cut.tile == 16) {
+                    e = attend_launch<T, E4, HD, 2>(c, a, grid, dev, st);
+                    return;
+                }
+            }
+            e = attend_launch<T, E4, HD, 1>(c, a, grid, dev, st);
         });
     });
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return op_error(LLMB_ERR_CUDA, "llm: %s: %s", what, cudaGetErrorString(e));
+    }
     if ((rc = op_launched(what)) != LLMB_OK || cut.splits == 1) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(((int64_t)c.max_new * heads + 7) / 8), 1, c.nseq);
+    const bool many = cut.splits > 8;
+    cfg.gridDim = dim3((unsigned)(many ? (int64_t)c.max_new * heads : ((int64_t)c.max_new * heads + 7) / 8), 1, c.nseq);
     cfg.blockDim = dim3(256);
     cfg.stream = st, cfg.attrs = &attr, cfg.numAttrs = 1;
     by_type(type, [&](auto t) {
         using T = decltype(t);
-        if (hd == 64) cudaLaunchKernelEx(&cfg, k_kv8_join<T, 64>, c, a);
-        else cudaLaunchKernelEx(&cfg, k_kv8_join<T, 128>, c, a);
+        if (hd == 64) many ? cudaLaunchKernelEx(&cfg, k_kv8_join<T, 64, 8>, c, a) : cudaLaunchKernelEx(&cfg, k_kv8_join<T, 64, 1>, c, a);
+        else many ? cudaLaunchKernelEx(&cfg, k_kv8_join<T, 128, 8>, c, a) : cudaLaunchKernelEx(&cfg, k_kv8_join<T, 128, 1>, c, a);
     });
     return op_launched(what);
 }

@@ -35,6 +35,7 @@
 
 #include "kv8.hpp"
 #include "kv8_chunk.hpp"
+#include "ops.hpp"
 
 namespace llmb {
 namespace {
@@ -671,26 +672,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
 }
 
 template <class T, bool E4M3, int HD>
-cudaError_t launch(const Kv8 &c, const Kv8Att &a, dim3 grid, cudaStream_t st) noexcept {
+cudaError_t launch(const Kv8 &c, const Kv8Att &a, dim3 grid, int device, cudaStream_t st) noexcept {
     constexpr int bytes = Layout<T, HD>::total;
-    const cudaError_t e = cudaFuncSetAttribute(k_kv8_chunk<T, E4M3, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-    k_kv8_chunk<T, E4M3, HD><<<grid, kThreads, bytes, st>>>(c, a);
-    return cudaSuccess;
+    const cudaError_t e = op_shared<k_kv8_chunk<T, E4M3, HD>>(device, bytes);
+    if (e == cudaSuccess) k_kv8_chunk<T, E4M3, HD><<<grid, kThreads, bytes, st>>>(c, a);
+    return e;
 }
 
 template <class T>
-cudaError_t launch(bool e4m3, int hd, const Kv8 &c, const Kv8Att &a, dim3 grid, cudaStream_t st) noexcept {
-    if (e4m3) return hd == 64 ? launch<T, true, 64>(c, a, grid, st) : launch<T, true, 128>(c, a, grid, st);
-    return hd == 64 ? launch<T, false, 64>(c, a, grid, st) : launch<T, false, 128>(c, a, grid, st);
+cudaError_t launch(bool e4m3, int hd, const Kv8 &c, const Kv8Att &a, dim3 grid, int device, cudaStream_t st) noexcept {
+    if (e4m3) return hd == 64 ? launch<T, true, 64>(c, a, grid, device, st) : launch<T, true, 128>(c, a, grid, device, st);
+    return hd == 64 ? launch<T, false, 64>(c, a, grid, device, st) : launch<T, false, 128>(c, a, grid, device, st);
 }
 
 }  // namespace
 
-cudaError_t kv8_chunk_launch(int type, bool e4m3, int hd, const Kv8 &c, const Kv8Att &a, dim3 grid, cudaStream_t st) noexcept {
-    if (type == LLMB_F32) return launch<float>(e4m3, hd, c, a, grid, st);
-    if (type == LLMB_F16) return launch<__half>(e4m3, hd, c, a, grid, st);
-    return launch<__nv_bfloat16>(e4m3, hd, c, a, grid, st);
+cudaError_t kv8_chunk_launch(int type, bool e4m3, int hd, const Kv8 &c, const Kv8Att &a, dim3 grid, int device,
+                             cudaStream_t st) noexcept {
+    if (type == LLMB_F32) return launch<float>(e4m3, hd, c, a, grid, device, st);
+    if (type == LLMB_F16) return launch<__half>(e4m3, hd, c, a, grid, device, st);
+    return launch<__nv_bfloat16>(e4m3, hd, c, a, grid, device, st);
 }
 
 }  // namespace llmb

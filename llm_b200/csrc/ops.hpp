@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <initializer_list>
 
@@ -33,5 +34,15 @@ int op_alignment(const char *what, std::initializer_list<OpPointer> ps) noexcept
 
 // The error of the launch just made (none was pending before it): cleared and reported.
 int op_launched(const char *what) noexcept;
+
+// Lets a kernel use that much dynamic shared memory, once per device (the call costs as much as a launch's checks).
+template <auto *Kernel>
+cudaError_t op_shared(int device, int bytes) noexcept {
+    static std::atomic<bool> done[64];
+    if (device < 64 && done[device].load(std::memory_order_relaxed)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device < 64) done[device].store(true, std::memory_order_relaxed);
+    return e;
+}
 
 }  // namespace llmb

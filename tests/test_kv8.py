@@ -68,7 +68,7 @@ def test_bad_rows_are_refused():
     assert _append(L, c, b, type_=3) == arg and _append(L, c, b, stride=124) == arg and _append(L, c, b, stride=130) == arg
     assert _append(L, c, b, type_=2, stride=132) == arg  # 264 bytes
     assert L.llmb_kv8_read(c, b, 4097, None, 0, 128, None) == arg
-    for bad in (dict(heads=13), dict(heads=0), dict(heads=2 * 65), dict(window=-1), dict(scale=math.inf),
+    for bad in (dict(heads=13), dict(heads=0), dict(heads=2 * 65), dict(window=-1), dict(scale=math.inf), dict(scale=-0.5),
                 dict(scale=math.nan), dict(qs=892), dict(os_=894), dict(q=None), dict(out=4104), dict(type_=-1)):
         assert _attend(L, c, b, **bad) == arg, bad
     assert b"attention" in L.llmb_last_error(None)
