@@ -27,18 +27,47 @@ constexpr float kFit = 1.f / 4096.f;        // a scale still fits top + kFit ste
 constexpr float kTiny = 7.888609052e-31f;   // 2^-100
 constexpr float kRestart = 1048576.f;       // 2^20
 
-// Four values to 8 bits: to the nearest, ties to even, saturated; NaN becomes 0.
-template <bool E4M3>
+// Four values to 8 bits: to the nearest, ties to even, saturated; NaN becomes 0.  FINITE: none of them is infinite or NaN
+// and none above the top by more than the scale's rounding, so that rounding alone ends at the top.
+template <bool E4M3, bool FINITE>
 __device__ __forceinline__ uint32_t kv8_pack(const float (&x)[4], float inv) {
-    uint32_t w = 0;
+    float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float y = __fmul_rn(x[i], inv);
-        y = y == y ? fminf(fmaxf(y, -kv8_top<E4M3>()), kv8_top<E4M3>()) : 0.f;
-        if (E4M3) w |= (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3) << (8 * i);
-        else w |= ((uint32_t)__float2int_rn(y) & 0xffu) << (8 * i);
+        y[i] = __fmul_rn(x[i], inv);
+        if (!FINITE) y[i] = y[i] == y[i] ? fminf(fmaxf(y[i], -kv8_top<E4M3>()), kv8_top<E4M3>()) : 0.f;
     }
-    return w;
+    if constexpr (E4M3) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        return lo | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+    } else {
+        // 1.5 2^23 + y: the rounded y is in the low bits (a conversion to int runs at a quarter of an addition's rate)
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fadd_rn(y[i], 12582912.f));
+        return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    }
+}
+
+// The largest magnitude's bits of the 16 bytes, in the upper half for 16-bit types: they order like the values, with
+// infinity and NaN above the finite ones (from kv8_inf on).
+template <class T>
+__device__ __forceinline__ uint32_t kv8_top_bits(const uint4 &r, uint32_t m) {
+    if (sizeof(T) == 4)
+        return max(max(max(m, r.x & 0x7fffffffu), r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+    return __vmaxu2(__vmaxu2(__vmaxu2(m, r.x & 0x7fff7fffu), __vmaxu2(r.y & 0x7fff7fffu, r.z & 0x7fff7fffu)), r.w & 0x7fff7fffu);
+}
+template <class T>
+constexpr uint32_t kv8_inf = 0x7f800000u;
+template <>
+constexpr uint32_t kv8_inf<__half> = 0x7c00u;
+template <>
+constexpr uint32_t kv8_inf<__nv_bfloat16> = 0x7f80u;
+template <class T>
+__device__ __forceinline__ float kv8_of_bits(uint32_t m) {
+    if (sizeof(T) == 4) return __uint_as_float(m);
+    const unsigned short h = (unsigned short)m;
+    return kv8_float<T>(*reinterpret_cast<const T *>(&h));
 }
 
 // A block's new scale from the largest magnitude a of the rows it receives
@@ -70,15 +99,17 @@ __device__ __forceinline__ void kv8_unpack(const uint4 &r, float (&x)[16 / sizeo
     for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[i] = kv8_float<T>(e[i]);
 }
 
-// One block and kv head of K or V: its new rows are held in registers (U
-// pieces of 16 bytes a thread) between the maximum and the rounding, so they
-// are read once.
+// One block of a sequence, and `tiles` of its 2 kv_heads tiles (K and V of one
+// head after the other): a tile's new rows are held in registers (U pieces of
+// 16 bytes a thread) between the maximum and the rounding, so they are read
+// once, and the next tile's are on their way meanwhile.  Bound by the memory's
+// rate; several tiles a block of threads spread the three look-ups (lengths,
+// table, scale) that come before the first load.
 template <class T, bool E4M3, int HD, int U>
 __global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__restrict__ k, const T *__restrict__ v,
-                                                    int64_t row_stride) {
+                                                    int64_t row_stride, int tiles) {
     constexpr int E = 16 / (int)sizeof(T), PR = HD / E;  // elements of a piece, pieces of a row
-    const int s = blockIdx.z, head = blockIdx.y >> 1;
-    const bool val = blockIdx.y & 1;
+    const int s = blockIdx.z;
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
     const int first = max(q.first, 0);
@@ -87,85 +118,123 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__rest
     const int b = kv8_block(c, s, j);
     if (b < 0) return;
     const int lo = max(first - p0, 0), hi = min(q.len - p0, c.block), total = (hi - lo) * PR;
-    const T *src = (val ? v : k) + (int64_t)(q.start + p0 + lo - q.first) * row_stride + head * HD;
-    uint8_t *tile = (val ? c.v : c.k) + b * c.bstride + (int64_t)head * c.block * HD;
-    float *scale = (val ? c.vs : c.ks) + (int64_t)b * c.kvh + head;
-    float s0 = lo > 0 ? *scale : 0.f;
-    uint4 x[U];
-    float a = 0.f;
+    const int64_t row = (int64_t)(q.start + p0 + lo - q.first) * row_stride;
+    const int t1 = min((int)(blockIdx.y + 1) * tiles, 2 * c.kvh);
+    __shared__ uint32_t red[2][8];
+    uint4 x[U], y[U];
+    float s0 = 0.f, s1 = 0.f;
+    auto load = [&](int t, uint4 (&r)[U], float &held) {  // tile t: head t / 2, V where t is odd
+        const T *src = (t & 1 ? v : k) + row + (t >> 1) * HD;
+        held = lo > 0 ? (t & 1 ? c.vs : c.ks)[(int64_t)b * c.kvh + (t >> 1)] : 0.f;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const int u = threadIdx.x + i * blockDim.x;
-        if (u < total) x[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)(u / PR) * row_stride + u % PR * E));
-    }
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * blockDim.x;
+            if (u < total) r[i] = __ldg(reinterpret_cast<const uint4 *>(src + (int64_t)(u / PR) * row_stride + u % PR * E));
+        }
+    };
+    auto store = [&](int t, const uint4 (&r)[U], float s0) {
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-        if ((int)(threadIdx.x + i * blockDim.x) < total) {
-            float f[E];
-            kv8_unpack<T>(x[i], f);
+        for (int i = 0; i < U; ++i)
+            if ((int)(threadIdx.x + i * blockDim.x) < total) m = kv8_top_bits<T>(r[i], m);
+        if (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
+        if (!(s0 > 0.f && s0 <= FLT_MAX)) s0 = 0.f;
+        m = __reduce_max_sync(kFull, m);
+        if ((threadIdx.x & 31) == 0) red[t & 1][threadIdx.x >> 5] = m;
+        __syncthreads();  // and every thread has read this tile's scale
+        for (int w = 0; w < (int)blockDim.x / 32; ++w) m = max(m, red[t & 1][w]);
+        const bool finite = m < kv8_inf<T>;
+        float a = kv8_of_bits<T>(m);
+        if (!finite) {  // the largest of the finite ones
+            a = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float m = fabsf(f[e]);
-                if (m <= FLT_MAX) a = fmaxf(a, m);
+            for (int i = 0; i < U; ++i)
+                if ((int)(threadIdx.x + i * blockDim.x) < total) {
+                    float f[E];
+                    kv8_unpack<T>(r[i], f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) a = fabsf(f[e]) <= FLT_MAX ? fmaxf(a, fabsf(f[e])) : a;
+                }
+            m = __reduce_max_sync(kFull, __float_as_uint(a));
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) red[t & 1][threadIdx.x >> 5] = m;
+            __syncthreads();
+            for (int w = 0; w < (int)blockDim.x / 32; ++w) m = max(m, red[t & 1][w]);
+            a = __uint_as_float(m);
+        }
+        float old;
+        const float sc = kv8_grow<E4M3>(a, s0, old);
+        if (s0 == 0.f) old = 0.f;  // rows without a scale are 0
+        uint8_t *tile = (t & 1 ? c.v : c.k) + b * c.bstride + (int64_t)(t >> 1) * c.block * HD;
+        if (threadIdx.x == 0) (t & 1 ? c.vs : c.ks)[(int64_t)b * c.kvh + (t >> 1)] = sc;
+        const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+        auto write = [&](auto all_finite) {
+            constexpr bool F = decltype(all_finite)::value;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int u = threadIdx.x + i * blockDim.x;
+                if (u < total) {
+                    float f[E];
+                    kv8_unpack<T>(r[i], f);
+                    uint32_t *dst = reinterpret_cast<uint32_t *>(tile + lo * HD + u * E);
+                    if constexpr (E == 4) {
+                        *dst = kv8_pack<E4M3, F>(f, inv);
+                    } else {
+                        const float f0[4] = {f[0], f[1], f[2], f[3]}, f1[4] = {f[4], f[5], f[6], f[7]};
+                        *reinterpret_cast<uint2 *>(dst) = make_uint2(kv8_pack<E4M3, F>(f0, inv), kv8_pack<E4M3, F>(f1, inv));
+                    }
+                }
             }
-        }
-    if (!(s0 > 0.f && s0 <= FLT_MAX)) s0 = 0.f;
-    __shared__ float red[8];
-    for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(kFull, a, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();  // and every thread has read the scale
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) a = fmaxf(a, red[w]);
-    float old;
-    const float sc = kv8_grow<E4M3>(a, s0, old);
-    if (s0 == 0.f) old = 0.f;  // rows without a scale are 0
-    if (threadIdx.x == 0) *scale = sc;
-    const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const int u = threadIdx.x + i * blockDim.x;
-        if (u < total) {
-            float f[E];
-            kv8_unpack<T>(x[i], f);
-            uint32_t *dst = reinterpret_cast<uint32_t *>(tile + lo * HD + u * E);
-            if constexpr (E == 4) {
-                *dst = kv8_pack<E4M3>(f, inv);
-            } else {
-                const float f0[4] = {f[0], f[1], f[2], f[3]}, f1[4] = {f[4], f[5], f[6], f[7]};
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(kv8_pack<E4M3>(f0, inv), kv8_pack<E4M3>(f1, inv));
+        };
+        finite ? write(std::true_type{}) : write(std::false_type{});
+        if (old != 1.f)
+            for (int u = threadIdx.x; u < lo * HD / 4; u += blockDim.x) {
+                uint32_t *w = reinterpret_cast<uint32_t *>(tile) + u;
+                float f[4];
+                kv8_floats<E4M3>(*w, f);
+                *w = kv8_pack<E4M3, false>(f, old);  // (a byte may be anything)
             }
-        }
+    };
+    int t = blockIdx.y * tiles;
+    if (t >= t1) return;
+    load(t, x, s0);
+    for (; t < t1; t += 2) {
+        if (t + 1 < t1) load(t + 1, y, s1);
+        store(t, x, s0);
+        if (t + 1 >= t1) break;
+        if (t + 2 < t1) load(t + 2, x, s0);
+        store(t + 1, y, s1);
     }
-    if (old != 1.f)
-        for (int u = threadIdx.x; u < lo * HD / 4; u += blockDim.x) {
-            uint32_t *w = reinterpret_cast<uint32_t *>(tile) + u;
-            float f[4];
-            kv8_floats<E4M3>(*w, f);
-            *w = kv8_pack<E4M3>(f, old);
-        }
+}
+
+// Tiles of a block that one block of threads takes: as many as spread its look-ups without leaving SMs idle.
+int tiles_each(const Kv8 &c, int64_t touched, int tile_bytes) {
+    const int64_t all = touched * c.nseq * 2 * c.kvh;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({all / (148 * 8), 2 * c.kvh, 65536 / tile_bytes}));
 }
 
 template <class T, bool E4M3, int HD>
 void append_launch(const Kv8 &c, const void *k, const void *v, int64_t row_stride, int touched, cudaStream_t st) {
-    const dim3 grid(touched, 2 * c.kvh, c.nseq);
+    const int tiles = tiles_each(c, touched, c.block * HD * (int)sizeof(T));
+    const dim3 grid(touched, (2 * c.kvh + tiles - 1) / tiles, c.nseq);
     const int pieces = min(c.max_new, c.block) * HD * (int)sizeof(T) / 16;
     const T *kp = static_cast<const T *>(k), *vp = static_cast<const T *>(v);
-    // (a block has at most 128 rows: HD sizeof(T) / 32 pieces for each of 256 threads)
     // the fewest threads that hold the rows with few pieces each: a decoding step's single row needs one warp
-    if (pieces <= 64) k_kv8_append<T, E4M3, HD, 2><<<grid, 32, 0, st>>>(c, kp, vp, row_stride);
-    else if (HD * (int)sizeof(T) <= 128 || pieces <= 1024) k_kv8_append<T, E4M3, HD, 4><<<grid, 256, 0, st>>>(c, kp, vp, row_stride);
-    else k_kv8_append<T, E4M3, HD, HD * (int)sizeof(T) / 32><<<grid, 256, 0, st>>>(c, kp, vp, row_stride);
+    // (a block has at most 128 rows: HD sizeof(T) / 32 pieces for each of 256 threads)
+    if (pieces <= 64) k_kv8_append<T, E4M3, HD, 2><<<grid, 32, 0, st>>>(c, kp, vp, row_stride, tiles);
+    else if (HD * (int)sizeof(T) <= 128 || pieces <= 1024) k_kv8_append<T, E4M3, HD, 4><<<grid, 256, 0, st>>>(c, kp, vp, row_stride, tiles);
+    else k_kv8_append<T, E4M3, HD, HD * (int)sizeof(T) / 32><<<grid, 256, 0, st>>>(c, kp, vp, row_stride, tiles);
 }
 
 // --------------------------------------------------------------- read --
 
-// One block and kv head of K or V, four values a thread and step.
+// One block of a sequence and `tiles` of its 2 kv_heads tiles, 16 bytes of
+// result a thread and step, four steps' loads in flight.
 template <class T, bool E4M3, int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k, T *__restrict__ v,
-                                                  int64_t row_stride) {
-    const int s = blockIdx.z, head = blockIdx.y >> 1;
-    const bool val = blockIdx.y & 1;
-    T *dst = val ? v : k;
-    if (!dst) return;
+                                                  int64_t row_stride, int tiles) {
+    constexpr int E = 16 / (int)sizeof(T), PR = HD / E, N = 4;  // values of a step, steps of a row, steps in flight
+    const int s = blockIdx.z;
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
     // blocks counted from the one that holds the first row's position, which may be below 0
@@ -173,22 +242,35 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
     if (p0 >= q.len) return;
     const int b = kv8_block(c, s, j);
     const int lo = max(q.first - p0, 0), hi = min(q.len - p0, c.block);
-    const uint8_t *tile = (val ? c.v : c.k) + (b < 0 ? 0 : b) * c.bstride + (int64_t)head * c.block * HD;
-    const float sc = b < 0 ? 0.f : (val ? c.vs : c.ks)[(int64_t)b * c.kvh + head];
-    dst += (int64_t)(q.start + p0 - q.first) * row_stride + head * HD;
-    for (int u = lo * (HD / 4) + threadIdx.x; u < hi * (HD / 4); u += blockDim.x) {
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (b >= 0) {
-            kv8_floats<E4M3>(__ldg(reinterpret_cast<const uint32_t *>(tile) + u), f);
+    const int64_t row = (int64_t)(q.start + p0 - q.first) * row_stride;
+    const int t0 = blockIdx.y * tiles, t1 = min(t0 + tiles, 2 * c.kvh), per = c.block * PR;
+    const int shift = c.bshift + (PR == 32 ? 5 : PR == 16 ? 4 : 3);  // of `per`, a power of two
+    for (int u0 = threadIdx.x; u0 < (t1 - t0) * per; u0 += N * blockDim.x) {
+        uint2 w[N];
+        float sc[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = __fmul_rn(f[i], sc);
+        for (int i = 0; i < N; ++i) {
+            const int u = u0 + i * blockDim.x, t = t0 + (u >> shift), e = u & (per - 1);
+            w[i] = make_uint2(0, 0), sc[i] = 0.f;
+            if (t < t1 && b >= 0) {
+                const uint8_t *src = (t & 1 ? c.v : c.k) + b * c.bstride + (int64_t)(t >> 1) * c.block * HD + e * E;
+                if constexpr (E == 8) w[i] = __ldg(reinterpret_cast<const uint2 *>(src));
+                else w[i].x = __ldg(reinterpret_cast<const uint32_t *>(src));
+                sc[i] = __ldg((t & 1 ? c.vs : c.ks) + (int64_t)b * c.kvh + (t >> 1));
+            }
         }
-        T *o = dst + (int64_t)(u / (HD / 4)) * row_stride + u % (HD / 4) * 4;
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(o) = make_float4(f[0], f[1], f[2], f[3]);
-        } else {
-            T h[4] = {kv8_from<T>(f[0]), kv8_from<T>(f[1]), kv8_from<T>(f[2]), kv8_from<T>(f[3])};
-            *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(h);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = u0 + i * blockDim.x, t = t0 + (u >> shift), e = u & (per - 1), r = e / PR;
+            T *dst = t & 1 ? v : k;
+            if (t >= t1 || r < lo || r >= hi || !dst) continue;
+            float f[4], h[4];
+            kv8_floats<E4M3>(w[i].x, f);
+            if (E == 8) kv8_floats<E4M3>(w[i].y, h);
+            T o[E];
+#pragma unroll
+            for (int z = 0; z < E; ++z) o[z] = kv8_from<T>(b < 0 ? 0.f : __fmul_rn(z < 4 ? f[z & 3] : h[z & 3], sc[i]));
+            *reinterpret_cast<uint4 *>(dst + row + (int64_t)r * row_stride + (t >> 1) * HD + e % PR * E) = *reinterpret_cast<const uint4 *>(o);
         }
     }
 }
@@ -285,6 +367,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
     constexpr int PIECES = kPieces<T>, ROWS = 8 * NB, KS = HD / 16, NT = HD / 16;  // k steps; tiles of 16 elements of V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int s = blockIdx.z, head = blockIdx.y % c.kvh, row0 = blockIdx.y / c.kvh * ROWS;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join waits for this kernel's end itself
     const Kv8Seq sq = kv8_seq(c, s);
     const int rows = sq.n * a.group;
     if (row0 >= rows) return;
@@ -609,12 +692,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
 template <class T, int HD, int W>
 __global__ void __launch_bounds__(256) k_kv8_join(const Kv8 c, const Kv8Att a) {
     constexpr int E = HD / 32;  // elements of a lane
-    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = blockIdx.z;
     const Kv8Seq sq = kv8_seq(c, s);
     const int64_t r = (int64_t)blockIdx.x * (8 / W) + warp / W;
     const bool on = r < (int64_t)sq.n * a.heads;
-    if (W == 1 && !on) return;
     const int tok = on ? (int)(r / a.heads) : 0, h = on ? (int)(r % a.heads) : 0, kvr = tok * a.group + h % a.group;
     // the span of the row's tile, as its parts were cut
     const int row0 = kvr / a.tile * a.tile, last = min(row0 + a.tile, sq.n * a.group) - 1;
@@ -625,6 +706,8 @@ __global__ void __launch_bounds__(256) k_kv8_join(const Kv8 c, const Kv8Att a) {
     float M = -FLT_MAX, L = 0.f, O[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) O[k] = 0.f;
+    // (what is read above was written before the attention began)
+    cudaGridDependencySynchronize();
     // the warp's parts are warp % W, + W, ...; a lane weighs one in 32
     for (int i0 = warp % W; i0 < parts; i0 += 32 * W) {
         const int mine = i0 + lane * W, n = min((parts - i0 + W - 1) / W, 32);
@@ -667,6 +750,7 @@ __global__ void __launch_bounds__(256) k_kv8_join(const Kv8 c, const Kv8Att a) {
             for (int k = 0; k < E; ++k) O[k] = fmaf(f, so[w][lane * E + k], O[k]);
         }
     }
+    if (!on) return;
     T v[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) v[k] = kv8_from<T>(L == 0.f ? 0.f : O[k] / L);
@@ -862,9 +946,10 @@ int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, void
     by_type(type, [&](auto t) {
         by_cache(cache->type, cache->head_dim, [&](auto e4m3, auto hd) {
             using T = decltype(t);
+            const int tiles = tiles_each(c, touched(c), c.block * decltype(hd)::value * (int)sizeof(T));
             k_kv8_read<T, decltype(e4m3)::value, decltype(hd)::value>
-                <<<dim3((unsigned)touched(c), 2 * c.kvh, c.nseq), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                    c, static_cast<T *>(k), static_cast<T *>(v), row_stride);
+                <<<dim3((unsigned)touched(c), (2 * c.kvh + tiles - 1) / tiles, c.nseq), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                    c, static_cast<T *>(k), static_cast<T *>(v), row_stride, tiles);
         });
     });
     return op_launched(what);

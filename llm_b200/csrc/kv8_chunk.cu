@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
     float *facs = reinterpret_cast<float *>(smem + L::fac);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int s = blockIdx.z, head = blockIdx.y % c.kvh, row0 = blockIdx.y / c.kvh * ROWS;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join waits for this kernel's end itself
     const Kv8Seq sq = kv8_seq(c, s);
     const int rows = sq.n * a.group;
     if (row0 >= rows) return;
