@@ -14,14 +14,15 @@
 // 32 tokens go round among them, so that the frequent tokens, which have low
 // ids, do not all fall to one.  A CTA counts the history's tokens among its
 // own in a table in shared memory, a 32-bit word per token: the count in bits
-// 13..31, bit 12 for the prompt's tokens, in bits 0..11 the place of the
+// 0..18, bit 19 for the prompt's tokens, in bits 20..31 the place of the
 // token's bias (1..4095).  Counts are integers and of a token's biases the
-// last counts, so the order of the atomics does not matter.  Whoever touches a
-// word first lists it; then each listed token's logit is worked out, left in
-// its word, and marked in a bitmap.  The pass over the logits has only the
-// bits to look at (working tokens out there cost 57 instructions a logit: a
-// warp meets one of the history in most of its 128).  The cluster's first CTA
-// takes the largest of the CTAs' maxima; the others do not wait for it.
+// last counts, so the order of the atomics does not matter.  The pass looks a
+// logit's word up and works out those that have one.  Bound by latency: a CTA
+// has about 10 K logits, so everything it reads first (logits, history,
+// biases, lengths) is asked for before the table is cleared, and there are
+// two barriers in all.  What is left of the time is instructions: 270 for 128
+// logits, a quarter of them divisions for single lanes.  The cluster's first CTA takes the largest of the CTAs'
+// maxima; the others do not wait for it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -39,8 +40,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kThreads = 512;
-constexpr int kMaxSlice = 11264;  // tokens of a CTA and round: 68 KiB with bitmap and list, three CTAs an SM
+constexpr int kThreads = 384;
+constexpr int kMaxSlice = 11264;  // tokens of a CTA and round: a table of 44 KiB
 constexpr int kMaxBias = 4095, kMaxHistory = (1 << 19) - 1;
 
 struct Ctl {
@@ -67,13 +68,11 @@ __device__ __forceinline__ uint64_t rank_of(float x, int v) {
 __device__ __forceinline__ uint32_t su32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
+__global__ void __launch_bounds__(kThreads, 4) k_logits(const Ctl c) {
     constexpr int E = 16 / (int)sizeof(T);
-    extern __shared__ __align__(16) uint32_t table[];  // c.slice words (a multiple of 32), their bitmap, the list
-    uint32_t *done = table + c.slice;
-    uint16_t *list = reinterpret_cast<uint16_t *>(done + c.slice / 32);
+    extern __shared__ __align__(16) uint32_t table[];  // c.slice words (a multiple of 32)
     __shared__ uint64_t best_w[kThreads / 32], best_c[16], bar;
-    __shared__ int listed;
+
     cg::cluster_group cluster = cg::this_cluster();
     const int nc = gridDim.x, rank = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int shift = 31 - __clz(nc);  // (a power of two)
@@ -82,12 +81,17 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(&bar)), "r"(nc));
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     }
     const T *in = static_cast<const T *>(c.logits) + (int64_t)row * c.stride;
     T *out = c.out ? static_cast<T *>(c.out) + (int64_t)row * c.out_stride : nullptr;
     const uint32_t *mask = c.mask ? c.mask + (int64_t)row * c.mask_stride : nullptr;
     const int *hist = c.history ? c.history + (int64_t)row * c.hist_stride : nullptr;
+    // the first ids of the thread, whether or not they will be wanted
+    constexpr int G = 4;
+    int ids[G], bias_id = -1;
+#pragma unroll
+    for (int k = 0; k < G; ++k) ids[k] = hist && tid + k * kThreads < c.hist_stride ? __ldg(hist + tid + k * kThreads) : -1;
     const int nh = hist ? min(max(c.hist_lens ? __ldg(c.hist_lens + row) : c.hist_stride, 0), c.hist_stride) : 0;
     const int np = c.prompt_lens ? __ldg(c.prompt_lens + row) : 0;
     float rep = 1.f, pres = 0.f, freq = 0.f;
@@ -98,6 +102,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
         bias0 = min(max(__ldg(c.bias_starts + row), 0), c.n_bias);
         bias1 = min(min(max(__ldg(c.bias_starts + row + 1), bias0), c.n_bias), bias0 + kMaxBias);
     }
+    if (bias0 + tid < bias1) bias_id = __ldg(c.bias_ids + bias0 + tid);
+    const bool controlled = nh > 0 || bias1 > bias0;
     float best_x = -INFINITY;
     int best_v = 0;
     for (int round = 0; round < c.rounds; ++round) {
@@ -109,8 +115,10 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
             const int j = (v >> (5 + shift)) - chunk0;
             return j >= 0 && j < c.slice / 32 ? j * 32 + (v & 31) : -1;
         };
-        auto load = [&](int u, uint4 &raw) {
+        auto load = [&](int u, uint4 &raw, uint32_t &bits) {
             const int v = token(u);
+            // E divides 32 and u is a multiple of E: one word of the mask
+            bits = mask && v < c.vocab ? __ldg(mask + (v >> 5)) >> (v & 31) : 0xffffffffu;
             if (VEC && v + E <= c.vocab) {
                 raw = *reinterpret_cast<const uint4 *>(in + v);
             } else {
@@ -123,66 +131,62 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
         constexpr int step = kThreads * E;
         // the first two vectors of the thread are on their way while the table is made
         uint4 r0, r1;
-        if (tid * E < c.slice) load(tid * E, r0);
-        if (tid * E + step < c.slice) load(tid * E + step, r1);
+        uint32_t b0, b1;
+        if (tid * E < c.slice) load(tid * E, r0, b0);
+        if (tid * E + step < c.slice) load(tid * E + step, r1, b1);
         if (round > 0) __syncthreads();
-        if (nh > 0 || bias1 > bias0)
+        if (controlled) {
             for (int i = 4 * tid; i < c.slice; i += 4 * kThreads) *reinterpret_cast<uint4 *>(table + i) = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < c.slice / 32; i += kThreads) done[i] = 0;
-        if (tid == 0) listed = 0;
-        __syncthreads();
-        // (whole warps go round, for the ballot)
-        auto enlist = [&](bool fresh, int off) {
-            const uint32_t m = __ballot_sync(kFull, fresh);
-            if (!m) return;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&listed, __popc(m));
-            at = __shfl_sync(kFull, at, 0) + __popc(m & ((1u << lane) - 1));
-            if (fresh) list[at] = (uint16_t)off;
-        };
-        if (bias1 > bias0) {
-            for (int i = bias0 + tid; i - lane < bias1; i += kThreads) {
-                const int off = i < bias1 ? place(__ldg(c.bias_ids + i)) : -1;
-                enlist(off >= 0 && atomicMax(table + off, (uint32_t)(i - bias0 + 1)) == 0, off);
-            }
+            __syncthreads();
+            auto bias = [&](int v, int i) {
+                const int off = place(v);
+                if (off < 0) return;
+                const uint32_t n = (uint32_t)(i - bias0 + 1);
+                for (uint32_t w = table[off], was; w >> 20 < n; w = was) {
+                    was = atomicCAS(table + off, w, n << 20 | (w & 0xfffffu));
+                    if (was == w) break;
+                }
+            };
+            auto count = [&](int v, int i) {
+                const int off = i < nh ? place(v) : -1;
+                if (off < 0) return;
+                if (i < np) atomicOr(table + off, 1u << 19);
+                else atomicAdd(table + off, 1u);
+            };
+            if (bias0 + tid < bias1) bias(bias_id, bias0 + tid);
+            for (int i = bias0 + tid + kThreads; i < bias1; i += kThreads) bias(__ldg(c.bias_ids + i), i);
+#pragma unroll
+            for (int k = 0; k < G; ++k) count(ids[k], tid + k * kThreads);
+#pragma unroll 4
+            for (int i = tid + G * kThreads; i < nh; i += kThreads) count(__ldg(hist + i), i);
             __syncthreads();
         }
-#pragma unroll 2
-        for (int i = tid; i - lane < nh; i += kThreads) {
-            const int off = i < nh ? place(__ldg(hist + i)) : -1;
-            uint32_t old = 1;
-            if (off >= 0) old = i < np ? atomicOr(table + off, 1u << 12) : atomicAdd(table + off, 1u << 13);
-            enlist(old == 0, off);
-        }
-        __syncthreads();
-        for (int i = tid; i < listed; i += kThreads) {
-            const int off = list[i];
-            const uint32_t w = table[off];
-            float y = kv8_float<T>(in[token(off)]);
-            if (w >> 12) {
+        auto controls = [&](float y, uint32_t w) {
+            if (w & 0xfffffu) {
+                const uint32_t n = w & 0x7ffffu;
                 y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                if (w >> 13) y = __fsub_rn(__fsub_rn(y, pres), __fmul_rn(freq, (float)(w >> 13)));
+                if (n) y = __fsub_rn(__fsub_rn(y, pres), __fmul_rn(freq, (float)n));
             }
-            if (w & 0xfffu) y = __fadd_rn(y, __ldg(c.bias_values + bias0 + (w & 0xfffu) - 1));
-            table[off] = __float_as_uint(y);
-            atomicOr(done + off / 32, 1u << (off % 32));
-        }
-        __syncthreads();
-        auto use = [&](int u, const uint4 &raw) {
+            if (w >> 20) y = __fadd_rn(y, __ldg(c.bias_values + bias0 + (w >> 20) - 1));
+            return y;
+        };
+        auto use = [&](int u, const uint4 &raw, uint32_t bits) {
             const T *e = reinterpret_cast<const T *>(&raw);
             const int v = token(u);
             if (v >= c.vocab) return;
             float x[E];
-            // E divides 32 and u is a multiple of E: one word of the mask and of the bitmap
-            uint32_t bits = mask ? __ldg(mask + (v >> 5)) >> (v & 31) : 0xffffffffu;
             if (v + E > c.vocab) bits &= (1u << (c.vocab - v)) - 1;
-            const uint32_t fixed = done[u >> 5] >> (u & 31) & ((1u << E) - 1);
 #pragma unroll
             for (int k = 0; k < E; ++k) x[k] = kv8_float<T>(e[k]);
-            if (fixed) {
+            if (controlled) {
 #pragma unroll
-                for (int k = 0; k < E; ++k)
-                    if (fixed >> k & 1) x[k] = __uint_as_float(table[u + k]);
+                for (int k = 0; k < E; k += 4) {
+                    const uint4 w4 = *reinterpret_cast<const uint4 *>(table + u + k);
+                    if (w4.x) x[k] = controls(x[k], w4.x);
+                    if (w4.y) x[k + 1] = controls(x[k + 1], w4.y);
+                    if (w4.z) x[k + 2] = controls(x[k + 2], w4.z);
+                    if (w4.w) x[k + 3] = controls(x[k + 3], w4.w);
+                }
             }
             T res[E];
 #pragma unroll
@@ -203,12 +207,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
         };
         for (int u = tid * E; u < c.slice; u += 2 * step) {
             const uint4 now = r0;
-            if (u + 2 * step < c.slice) load(u + 2 * step, r0);
-            use(u, now);
+            const uint32_t now_b = b0;
+            if (u + 2 * step < c.slice) load(u + 2 * step, r0, b0);
+            use(u, now, now_b);
             if (u + step >= c.slice) break;
             const uint4 next = r1;
-            if (u + 3 * step < c.slice) load(u + 3 * step, r1);
-            use(u + step, next);
+            const uint32_t next_b = b1;
+            if (u + 3 * step < c.slice) load(u + 3 * step, r1, b1);
+            use(u + step, next, next_b);
         }
     }
     if (!c.tokens) return;
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_logits(const Ctl c) {
     c.tokens[row] = ok && best ? (int32_t)~(uint32_t)best : -1;
 }
 
-constexpr size_t slice_bytes(int slice) { return (size_t)slice * 4 + slice / 8 + (size_t)slice * 2; }
+constexpr size_t slice_bytes(int slice) { return (size_t)slice * 4; }
 
 // Clusters of 16 CTAs are above the portable size and the table above the default's; each kernel is told so once per device.
 template <class T, bool VEC>
@@ -311,9 +317,11 @@ extern "C" int llmb_logits_control(const void *logits, int64_t stride, int type,
     if (rc == LLMB_OK) rc = op_pointers(what, dev, ps);
     if (rc != LLMB_OK) return rc;
     if (rows == 0) return LLMB_OK;
-    // one vector of a thread is the least that a CTA is worth launching for
+    // One vector of a thread is the least that a CTA is worth launching for.  Few rows take 16 CTAs each; with many, places
+    // for 8 at once are free sooner (64 rows of 151936: 38 us, with 16: 45 us, although the history is then read twice).
+    const int most = rows * 16 <= 2 * 148 ? 16 : 8;
     int ctas = 1;
-    while (ctas < 16 && ctas * kThreads * 16 / es < vocab) ctas *= 2;
+    while (ctas < most && ctas * kThreads * 16 / es < vocab) ctas *= 2;
     Ctl c{};
     const int chunks = (vocab + 32 * ctas - 1) / (32 * ctas);  // of 32 tokens, for each CTA
     c.rounds = (chunks + kMaxSlice / 32 - 1) / (kMaxSlice / 32);
