@@ -357,6 +357,30 @@ LLMB_API int llmb_logits_control(const void *logits, int64_t stride, int type, i
                                  const llmb_logits_ctl *ctl, void *out, int64_t out_stride, int32_t *tokens,
                                  void *stream);
 
+/* Called before each token is chosen, with the n tokens generated so far:
+ * sets the bit of every token that may come next in mask ((vocab + 31) / 32
+ * words; their contents are undefined before) and returns nonzero, or returns
+ * 0 to stop. */
+typedef int (*llmb_mask_fn)(void *user, const int32_t *tokens, int n, uint32_t *mask);
+
+/* The controls of llmb_generate_controlled, in host memory. */
+typedef struct {
+    float repetition, presence, frequency; /* as llmb_logits_ctl's penalties (1, 0, 0: none); repetition above 0 */
+    int32_t n_bias;                        /* at most 4095 */
+    const int32_t *bias_ids;               /* in the vocabulary; of a token's biases the last counts */
+    const float *bias_values;              /* -INFINITY forbids a token */
+    llmb_mask_fn mask;                     /* NULL: every token is allowed */
+    void *mask_user;
+} llmb_controls;
+
+/* llmb_generate with llmb_logits_control between the model's logits and each
+ * token (the prompt and the answer so far are the history).  Stops as
+ * Generate does, and where no token is allowed.  One token per launch, each
+ * read back before the next. */
+LLMB_API int llmb_generate_controlled(llmb_model *m, const int32_t *prompt, int n_prompt, int n, int32_t eos,
+                                      const llmb_controls *controls, llmb_emit_fn emit, void *user,
+                                      int32_t *out_tokens, int *n_out, llmb_timing *tm);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,7 +33,8 @@ EXPORTS = ("llmb_open", "llmb_open_reader", "llmb_close", "llmb_last_error", "ll
            "llmb_get_stats", "llmb_generate", "llmb_generate_batch", "llmb_prefill_logits", "llmb_generate_logits",
            "llmb_peek",
            "llmb_set_layers", "llmb_set_knob", "llmb_get_knob", "llmb_attention_noalloc", "llmb_kv8_append",
-           "llmb_kv8_read", "llmb_kv8_attention", "llmb_kv8_attention_workspace", "llmb_logits_control")
+           "llmb_kv8_read", "llmb_kv8_attention", "llmb_kv8_attention_workspace", "llmb_logits_control",
+           "llmb_generate_controlled")
 
 F32, F16, BF16 = range(3)            # types of rows and logits
 KV8_INT8, KV8_E4M3 = range(2)        # types of the 8-bit cache
@@ -79,6 +80,15 @@ class _LogitsCtl(C.Structure):
                [("mask_stride", C.c_int32)]
 
 
+MASK_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.POINTER(C.c_uint32))
+
+
+class _Controls(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("repetition", "presence", "frequency")] + \
+               [("n_bias", C.c_int32), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("mask", MASK_FN),
+                ("mask_user", C.c_void_p)]
+
+
 READ_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64)
 EMIT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int32)
 
@@ -104,6 +114,9 @@ def lib() -> C.CDLL:
         L.llmb_generate.restype = I
         L.llmb_generate_batch.argtypes = [P, P, P, I, I, C.c_int32, P, P, C.POINTER(_Timing)]
         L.llmb_generate_batch.restype = I
+        L.llmb_generate_controlled.argtypes = [P, P, I, I, C.c_int32, C.POINTER(_Controls), EMIT_FN, P, P, C.POINTER(I),
+                                               C.POINTER(_Timing)]
+        L.llmb_generate_controlled.restype = I
         L.llmb_prefill_logits.argtypes, L.llmb_prefill_logits.restype = [P, P, I, P], I
         L.llmb_generate_logits.argtypes, L.llmb_generate_logits.restype = [P, P, I, I, P, P], I
         L.llmb_peek.argtypes, L.llmb_peek.restype = [P, C.c_char_p, P, I], I
@@ -275,6 +288,47 @@ class GPU:
                    tm.record_ms, tm.submit_ms, tm.gpu_prefill_ms, tm.gpu_decode_ms, tm.decode_kernel_ms,
                    tm.decode_launches)
         return [out[i, : n_out[i]].copy() for i in range(len(ps))], t
+
+    def generate_controlled(self, prompt, n: int, eos: int = -1, repetition: float = 1.0, presence: float = 0.0,
+                            frequency: float = 0.0, biases: dict | None = None, mask=None,
+                            emit=None) -> tuple[np.ndarray, Timing]:
+        """Greedy decoding with penalties for repeated tokens, biases {token: value} and a grammar
+        (llmb_generate_controlled): mask(tokens, allowed) is given the tokens so far (int32) and the mask to fill
+        (uint32, bit v % 32 of word v / 32 is token v) and returns whether to go on. An exception of mask or emit
+        stops the generation and is raised."""
+        p = np.ascontiguousarray(prompt, np.int32)
+        out = np.zeros(max(n, 1), np.int32)
+        ids = np.array(list(biases or {}), np.int32)
+        values = np.array(list((biases or {}).values()), np.float32)
+        raised = []
+        words = (self.cfg.vocab + 31) // 32
+
+        def guarded(f):
+            def call(*a):
+                try:
+                    return 1 if f(*a) else 0
+                except BaseException as e:
+                    raised.append(e)
+                    return 0
+            return call
+
+        mask_fn, emit_fn = MASK_FN(), EMIT_FN()
+        if mask is not None:
+            mask_fn = MASK_FN(guarded(lambda _u, t, k, w: mask(
+                np.ctypeslib.as_array(t, (k,)).copy() if k else np.zeros(0, np.int32), np.ctypeslib.as_array(w, (words,)))))
+        if emit is not None:
+            emit_fn = EMIT_FN(guarded(lambda _u, t: emit(int(t))))
+        c = _Controls(repetition, presence, frequency, len(ids), ids.ctypes.data, values.ctypes.data, mask_fn, None)
+        n_out, tm = C.c_int(), _Timing()
+        rc = lib().llmb_generate_controlled(self._h, _ptr(p), len(p), n, eos, c, emit_fn, None, _ptr(out),
+                                            C.byref(n_out), C.byref(tm))
+        if raised:
+            raise raised[0]
+        self._check(rc)
+        t = Timing(tm.prefill_ms, tm.decode_ms, tm.prompt_tokens, tm.generated, tm.submits, tm.dispatches,
+                   tm.record_ms, tm.submit_ms, tm.gpu_prefill_ms, tm.gpu_decode_ms, tm.decode_kernel_ms,
+                   tm.decode_launches)
+        return out[: n_out.value].copy(), t
 
     def prefill_logits(self, prompt) -> np.ndarray:
         """The logits of the prompt's last token (PrefillLogits, gpu.go:904)."""

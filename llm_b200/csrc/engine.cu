@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <chrono>
 #include <cmath>
 #include <cstring>
@@ -81,6 +82,8 @@ struct Model {
     TokBatch *h_tb = nullptr;
     float *bkv = nullptr;         // multi-stream: the KV arena, bkv_slots sequences
     int bkv_slots = 0;
+    uint8_t *ctl = nullptr;       // controlled generation: ControlBuffer and mask words (device), their pinned copy
+    uint8_t *h_ctl = nullptr;
     int64_t ll_tokens = 0;        // tokens the persistent kernel decoded since its tags were last reset
     // the m-token layer sequences (embedding + every layer's launches), captured once per
     // (tokens, batch or single sequence, layers) and replayed: a step of 64 sequences is ~210 launches
@@ -95,6 +98,7 @@ struct Model {
         for (void *p : allocs) cudaFree(p);
         if (h_tokens) cudaFreeHost(h_tokens);
         if (h_tb) cudaFreeHost(h_tb);
+        if (h_ctl) cudaFreeHost(h_ctl);
         for (auto &g : graphs) cudaGraphExecDestroy(g.second);
         if (h_state) cudaFreeHost(h_state);
         if (h_err) cudaFreeHost(h_err);
@@ -928,6 +932,103 @@ Error generate_logits(Model &m, const int32_t *prompt, int np, int n, int32_t *t
     return err;
 }
 
+// What llmb_logits_control reads on the device, followed by the mask's words.
+struct ControlBuffer {
+    float penalties[3];
+    int32_t prompt_len;
+    int32_t bias_ids[4096];
+    float bias_values[4096];
+};
+
+// Generate (gpu.go:941-1014) with llmb_logits_control choosing each token in
+// place of the largest logit: the control overwrites the token that the head
+// put at the sequence's end, from which the next launch starts.
+Error generate_controlled(Model &m, const int32_t *prompt, int np, int n, int32_t eos, const llmb_controls *ctl,
+                          llmb_emit_fn emit, void *user, int32_t *out_tokens, int *n_out, llmb_timing *tm_out) {
+    llmb_timing tm{};
+    if (n_out) *n_out = 0;
+    if (!ctl) return {LLMB_ERR_ARG, "llm: no controls"};
+    if (n < 0) return {LLMB_ERR_ARG, "llm: negative token count"};
+    if ((int64_t)np + n > m.cfg.ctx)
+        return {LLMB_ERR_CONTEXT, "llm: prompt of " + std::to_string(np) + " tokens and " + std::to_string(n) +
+                                      " new tokens exceed the context of " + std::to_string(m.cfg.ctx)};
+    Error err = check_prompt(m, prompt, np);
+    if (err.code) return err;
+    if (layers_to_run(m) != m.cfg.layers) return {LLMB_ERR_ARG, "llm: generation needs every layer"};
+    if (!(ctl->repetition > 0.f && ctl->repetition <= FLT_MAX) || !(std::fabs(ctl->presence) <= FLT_MAX) ||
+        !(std::fabs(ctl->frequency) <= FLT_MAX))
+        return {LLMB_ERR_ARG, "llm: penalties must be finite, and repetition above 0"};
+    if (ctl->n_bias < 0 || ctl->n_bias > 4095 || (ctl->n_bias > 0 && (!ctl->bias_ids || !ctl->bias_values)))
+        return {LLMB_ERR_ARG, "llm: " + std::to_string(ctl->n_bias) + " biases (at most 4095, ids and values)"};
+    for (int i = 0; i < ctl->n_bias; i++)
+        if (ctl->bias_ids[i] < 0 || ctl->bias_ids[i] >= m.cfg.vocab || std::isnan(ctl->bias_values[i]))
+            return {LLMB_ERR_ARG, "llm: bias " + std::to_string(i) + " is NaN or of no token"};
+    const size_t words = ((size_t)m.cfg.vocab + 31) / 32, bytes = sizeof(ControlBuffer) + words * 4;
+    if (!m.ctl && !(m.ctl = m.alloc<uint8_t>(bytes, err))) return err;
+    if (!m.h_ctl) CUDA_TRY(cudaHostAlloc(&m.h_ctl, bytes, cudaHostAllocDefault));
+    ControlBuffer &h = *reinterpret_cast<ControlBuffer *>(m.h_ctl), &d = *reinterpret_cast<ControlBuffer *>(m.ctl);
+    uint32_t *h_mask = reinterpret_cast<uint32_t *>(m.h_ctl + sizeof(ControlBuffer));
+    uint32_t *d_mask = reinterpret_cast<uint32_t *>(m.ctl + sizeof(ControlBuffer));
+    h.penalties[0] = ctl->repetition, h.penalties[1] = ctl->presence, h.penalties[2] = ctl->frequency;
+    h.prompt_len = np;
+    std::copy_n(ctl->bias_ids, ctl->n_bias, h.bias_ids);
+    std::copy_n(ctl->bias_values, ctl->n_bias, h.bias_values);
+    CUDA_TRY(cudaMemcpyAsync(m.ctl, m.h_ctl, sizeof(ControlBuffer), cudaMemcpyHostToDevice, m.st));
+
+    std::vector<int32_t> tokens;
+    tokens.reserve(n);
+    const int64_t s0 = m.stats.submits, d0 = m.stats.dispatches;
+    const double t0 = now_ms();
+    double t1 = t0;
+    CUDA_TRY(cudaEventRecord(m.ev0, m.st));
+    if ((err = begin(m, prompt, np)).code) return err;
+    if ((err = prefill(m, np)).code) return err;
+    CUDA_TRY(cudaEventRecord(m.ev1, m.st));
+    CUDA_TRY(cudaEventRecord(m.ev2, m.st));
+    tm.prompt_tokens = np;
+    for (int i = 0; i < n; i++) {
+        if (i > 0) {
+            if ((err = decode(m, 1)).code) return err;
+            tm.decode_launches++;
+        }
+        // (the mask is worked out while the model runs)
+        if (ctl->mask && !ctl->mask(ctl->mask_user, tokens.data(), (int)tokens.size(), h_mask)) break;
+        if (ctl->mask) CUDA_TRY(cudaMemcpyAsync(d_mask, h_mask, words * 4, cudaMemcpyHostToDevice, m.st));
+        llmb_logits_ctl c{};
+        c.history = m.hdm.tokens, c.history_stride = np + i, c.prompt_lens = &d.prompt_len, c.penalties = d.penalties;
+        if (ctl->n_bias > 0) c.n_bias = ctl->n_bias, c.bias_ids = d.bias_ids, c.bias_values = d.bias_values;
+        if (ctl->mask) c.mask = d_mask, c.mask_stride = (int32_t)words;
+        const int rc = llmb_logits_control(m.hdm.logits, m.cfg.vocab, LLMB_F32, 1, m.cfg.vocab, &c, nullptr, 0,
+                                           m.hdm.tokens + np + i, m.st);
+        if (rc != LLMB_OK) return {rc, t_open_error};
+        m.stats.dispatches++;
+        CUDA_TRY(cudaMemcpyAsync(m.h_tokens, m.hdm.tokens + np + i, 4, cudaMemcpyDeviceToHost, m.st));
+        CUDA_TRY(cudaMemcpyAsync(m.h_err, m.hdm.err, 4, cudaMemcpyDeviceToHost, m.st));
+        CUDA_TRY(cudaStreamSynchronize(m.st));
+        if ((err = device_status(m)).code) return err;
+        if (i == 0) tm.prefill_ms = now_ms() - t0, t1 = now_ms();
+        const int32_t tok = m.h_tokens[0];
+        if (tok < 0 || tok == eos) break;  // below 0: no token is allowed
+        tokens.push_back(tok);
+        if (out_tokens) out_tokens[i] = tok;
+        tm.generated++;
+        m.stats.tokens++;
+        if (emit && !emit(user, tok)) break;
+    }
+    CUDA_TRY(cudaEventRecord(m.ev3, m.st));
+    CUDA_TRY(cudaEventSynchronize(m.ev3));  // (a launch that a stop left behind, too)
+    if ((err = check_device(m)).code) return err;
+    tm.decode_ms = now_ms() - t1;
+    float a = 0, b = 0;
+    cudaEventElapsedTime(&a, m.ev0, m.ev1);
+    cudaEventElapsedTime(&b, m.ev2, m.ev3);
+    tm.gpu_prefill_ms = a, tm.gpu_decode_ms = b;
+    tm.submits = m.stats.submits - s0, tm.dispatches = m.stats.dispatches - d0;
+    if (n_out) *n_out = tm.generated;
+    if (tm_out) *tm_out = tm;
+    return {LLMB_OK, ""};
+}
+
 // Peek, gpu.go:1016-1043.
 Error peek(Model &m, const char *name, float *out, int n) {
     const DevModel &d = m.hdm;
@@ -1090,6 +1191,19 @@ int llmb_generate_logits(llmb_model *mp, const int32_t *prompt, int n_prompt, in
     Model *m = M(mp);
     cudaSetDevice(m->device);
     return fail(m, generate_logits(*m, prompt, n_prompt, n, out_tokens, step_logits));
+}
+
+int llmb_generate_controlled(llmb_model *mp, const int32_t *prompt, int n_prompt, int n, int32_t eos,
+                             const llmb_controls *controls, llmb_emit_fn emit, void *user, int32_t *out_tokens,
+                             int *n_out, llmb_timing *tm) {
+    if (!mp) return LLMB_ERR_ARG;
+    Model *m = M(mp);
+    cudaSetDevice(m->device);
+    try {
+        return fail(m, generate_controlled(*m, prompt, n_prompt, n, eos, controls, emit, user, out_tokens, n_out, tm));
+    } catch (const std::exception &) {  // no memory for the tokens
+        return LLMB_ERR_MEMORY;
+    }
 }
 
 int llmb_peek(llmb_model *mp, const char *name, float *out, int n) {
