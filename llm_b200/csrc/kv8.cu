@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
 
 // ---------------------------------------------------------- attention --
 
-constexpr int kAttWarps = 8;
+constexpr int kAttWarps = 4;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -324,7 +324,7 @@ struct Place {
 // (S^T = K Q^T, O^T = V^T P^T), so the few rows fill the 8 columns and each
 // value of the cache is converted once.
 //
-// A warp takes every 8th group of 16 positions, the next ones on their way
+// A warp takes every 4th group of 16 positions, the next ones on their way
 // (asynchronous copies) while one is worked on.  The contraction's index may
 // be permuted as long as both operands agree, so lane (g, t) = (lane / 4,
 // lane % 4) copies 16 contiguous bytes of the K rows g and g + 8 and uses them
@@ -348,8 +348,10 @@ constexpr int kPieces = 2;
 template <>
 constexpr int kPieces<__nv_bfloat16> = 1;
 
-// Groups of a warp in flight, as many as two CTAs an SM have room for (a group is 32 HD bytes), and their bytes.
-__host__ __device__ constexpr int att_depth(int hd) { return hd == 64 ? 5 : 3; }
+// Groups of a warp in flight, as many as four CTAs an SM have room for (a group is 32 HD bytes), and their bytes.
+__host__ __device__ constexpr int att_depth(int hd) { return hd == 64 ? 6 : 3; }
+// Groups worked on at once: two where the registers of four CTAs an SM hold them.
+__host__ __device__ constexpr int att_groups(int hd, int nb) { return hd == 64 && nb == 1 ? 2 : 1; }
 __host__ __device__ constexpr int att_smem(int hd) { return kAttWarps * att_depth(hd) * 32 * hd; }
 
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
@@ -363,7 +365,7 @@ template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <class T, bool E4M3, int HD, int NB>
-__global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(const Kv8 c, const Kv8Att a) {
+__global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 4 : 2) k_kv8_attend(const Kv8 c, const Kv8Att a) {
     constexpr int PIECES = kPieces<T>, ROWS = 8 * NB, KS = HD / 16, NT = HD / 16;  // k steps; tiles of 16 elements of V
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int s = blockIdx.z, head = blockIdx.y % c.kvh, row0 = blockIdx.y / c.kvh * ROWS;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
     };
     // the first groups are on their way before the queries are read
 #pragma unroll
-    for (int i = 0; i < D - 1; ++i) copy();
+    for (int i = 0; i < D - att_groups(HD, NB); ++i) copy();
 
     // the rows' queries as B fragments: row g of each 8
     uint32_t qf[NB][PIECES][KS][2];
@@ -500,49 +502,65 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
         m[i][0] = m[i][1] = -FLT_MAX, l[i][0] = l[i][1] = 0.f;
     }
 
-    auto use = [&](Group &x, int p0) {
-        const bool whole = p0 >= all0 && p0 + 16 <= all1;
-        float sc[NB][4];
+    // G groups at once: their chains of products and exponentials do not wait for one another.
+    auto use = [&](auto groups, Group *x, int p0) {
+        constexpr int G = decltype(groups)::value;
+        bool whole = true;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+        for (int y = 0; y < G; ++y) whole = whole && p0 + y * step >= all0 && p0 + y * step + 16 <= all1;
+        float sc[G][NB][4];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            uint32_t k0[2], k1[2];
-            auto word = [&](const uint4 &w) { return ks % 4 == 0 ? w.x : ks % 4 == 1 ? w.y : ks % 4 == 2 ? w.z : w.w; };
-            halves<E4M3>(word(x.k[0][ks / 4]), k0[0], k1[0]);
-            halves<E4M3>(word(x.k[1][ks / 4]), k0[1], k1[1]);
+        for (int y = 0; y < G; ++y)
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int i = 0; i < NB; ++i) sc[y][i][0] = sc[y][i][1] = sc[y][i][2] = sc[y][i][3] = 0.f;
 #pragma unroll
-                for (int q = PIECES - 1; q >= 0; --q) mma16816(sc[i], k0[0], k0[1], k1[0], k1[1], qf[i][q][ks]);
-        }
-        // sc[e]: position p0 + g + 8 (e / 2), row 2t + e % 2
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int y = 0; y < G; ++y) {
+                uint32_t k0[2], k1[2];
+                auto word = [&](const uint4 &w) { return ks % 4 == 0 ? w.x : ks % 4 == 1 ? w.y : ks % 4 == 2 ? w.z : w.w; };
+                halves<E4M3>(word(x[y].k[0][ks / 4]), k0[0], k1[0]);
+                halves<E4M3>(word(x[y].k[1][ks / 4]), k0[1], k1[1]);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int q = PIECES - 1; q >= 0; --q) mma16816(sc[y][i], k0[0], k0[1], k1[0], k1[1], qf[i][q][ks]);
+            }
+        // sc[.][.][e]: position p0 + g + 8 (e / 2), row 2t + e % 2
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int y = 0; y < G; ++y) {
+                const int p1 = p0 + y * step;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int q = p0 + g + 8 * (e >> 1);
-                    const bool seen = q <= pos[i][e & 1] && q < hi && (a.window == 0 || q > pos[i][e & 1] - a.window);
-                    if (!seen) sc[i][e] = -INFINITY;
-                }
-            // a byte behind the sequence's end may be a NaN of e4m3, which a weight of 0 would not stop
+                for (int i = 0; i < NB; ++i)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                if (p0 + 2 * t + (n & 1) + 8 * (n >> 1) >= hi)
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = p1 + g + 8 * (e >> 1);
+                        const bool seen = q <= pos[i][e & 1] && q < hi && (a.window == 0 || q > pos[i][e & 1] - a.window);
+                        if (!seen) sc[y][i][e] = -INFINITY;
+                    }
+                // a byte behind the sequence's end may be a NaN of e4m3, which a weight of 0 would not stop
 #pragma unroll
-                    for (int j = 0; j < HD / 32; ++j) x.v[n][j] = 0;
+                for (int n = 0; n < 4; ++n)
+                    if (p1 + 2 * t + (n & 1) + 8 * (n >> 1) >= hi)
+#pragma unroll
+                        for (int j = 0; j < HD / 32; ++j) x[y].v[n][j] = 0;
+            }
         }
-        float f[NB][2];
+        float f[G][NB][2], top[NB][2];
         bool up = false;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                f[i][e] = fac[i][e] * x.at.ks;
-                const float top = fmaxf(sc[i][e], sc[i][2 + e]);
-                // scores in log2, V's exponent added (a position not seen and a factor 0: -inf * 0 is NaN, not above)
-                up |= fmaf(top, f[i][e], x.at.lv) - m[i][e] > 8.f;
+                top[i][e] = -FLT_MAX;
+#pragma unroll
+                for (int y = 0; y < G; ++y) {
+                    f[y][i][e] = fac[i][e] * x[y].at.ks;
+                    // scores in log2, V's exponent added (a position not seen and a factor 0: -inf * 0 is NaN, passed over)
+                    top[i][e] = fmaxf(top[i][e], fmaf(fmaxf(sc[y][i][e], sc[y][i][2 + e]), f[y][i][e], x[y].at.lv));
+                }
+                up |= top[i][e] - m[i][e] > 8.f;
             }
         if (__any_sync(kFull, up)) {
 #pragma unroll
@@ -550,8 +568,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
                 float r[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float top = fmaxf(sc[i][e], sc[i][2 + e]);
-                    float n = top > -INFINITY ? fmaf(top, f[i][e], x.at.lv) : -FLT_MAX;
+                    float n = top[i][e];
                     n = fmaxf(n, __shfl_xor_sync(kFull, n, 4));
                     n = fmaxf(n, __shfl_xor_sync(kFull, n, 8));
                     n = fmaxf(n, __shfl_xor_sync(kFull, n, 16));
@@ -564,61 +581,57 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
                 for (int j = 0; j < NT; ++j) o[i][j][0] *= r[0], o[i][j][1] *= r[1], o[i][j][2] *= r[0], o[i][j][3] *= r[1];
             }
         }
-        uint32_t pf[NB][PIECES][2];
+        uint32_t pf[G][NB][PIECES][2];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            float w[4];
+        for (int y = 0; y < G; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = kv8_exp2(fmaf(sc[i][e], f[i][e & 1], x.at.lv + 6.f - m[i][e & 1]));
-                if (!whole && sc[i][e] == -INFINITY) w[e] = 0.f;
-            }
-            l[i][0] = fmaf(w[0] + w[2], x.at.unlv, l[i][0]), l[i][1] = fmaf(w[1] + w[3], x.at.unlv, l[i][1]);
+            for (int i = 0; i < NB; ++i) {
+                float w[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float w0 = w[2 * h] * x.at.mv, w1 = w[2 * h + 1] * x.at.mv;
-                const uint32_t y = pack_half2(w0, w1);
-                pf[i][0][h] = transpose8(y);
-                if constexpr (PIECES == 2) {
-                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&y));
-                    pf[i][1][h] = transpose8(pack_half2(w0 - b.x, w1 - b.y));
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = kv8_exp2(fmaf(sc[y][i][e], f[y][i][e & 1], x[y].at.lv + 6.f - m[i][e & 1]));
+                    if (!whole && sc[y][i][e] == -INFINITY) w[e] = 0.f;
+                }
+                l[i][0] = fmaf(w[0] + w[2], x[y].at.unlv, l[i][0]), l[i][1] = fmaf(w[1] + w[3], x[y].at.unlv, l[i][1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float w0 = w[2 * h] * x[y].at.mv, w1 = w[2 * h + 1] * x[y].at.mv;
+                    const uint32_t z = pack_half2(w0, w1);
+                    pf[y][i][0][h] = transpose8(z);
+                    if constexpr (PIECES == 2) {
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&z));
+                        pf[y][i][1][h] = transpose8(pack_half2(w0 - b.x, w1 - b.y));
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < NT; j += 2) {
-            // tiles j and j + 1 are the bytes 0, 1 and 2, 3 of word j / 2 of each V row
-            const uint32_t v0 = x.v[0][j / 2], v1 = x.v[1][j / 2], v2 = x.v[2][j / 2], v3 = x.v[3][j / 2];
-            uint32_t a0[2], a1[2], b0[2], b1[2];
-            halves<E4M3>(__byte_perm(v0, v1, 0x5140), a0[0], a0[1]);  // byte 0 and byte 1 of rows 2t, 2t + 1
-            halves<E4M3>(__byte_perm(v0, v1, 0x7362), a1[0], a1[1]);
-            halves<E4M3>(__byte_perm(v2, v3, 0x5140), b0[0], b0[1]);
-            halves<E4M3>(__byte_perm(v2, v3, 0x7362), b1[0], b1[1]);
+        for (int j = 0; j < NT; j += 2)
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int y = 0; y < G; ++y) {
+                // tiles j and j + 1 are the bytes 0, 1 and 2, 3 of word j / 2 of each V row
+                const uint32_t v0 = x[y].v[0][j / 2], v1 = x[y].v[1][j / 2], v2 = x[y].v[2][j / 2], v3 = x[y].v[3][j / 2];
+                uint32_t a0[2], a1[2], b0[2], b1[2];
+                halves<E4M3>(__byte_perm(v0, v1, 0x5140), a0[0], a0[1]);  // byte 0 and byte 1 of rows 2t, 2t + 1
+                halves<E4M3>(__byte_perm(v0, v1, 0x7362), a1[0], a1[1]);
+                halves<E4M3>(__byte_perm(v2, v3, 0x5140), b0[0], b0[1]);
+                halves<E4M3>(__byte_perm(v2, v3, 0x7362), b1[0], b1[1]);
 #pragma unroll
-                for (int q = PIECES - 1; q >= 0; --q) {
-                    mma16816(o[i][j], a0[0], a0[1], b0[0], b0[1], pf[i][q]);
-                    mma16816(o[i][j + 1], a1[0], a1[1], b1[0], b1[1], pf[i][q]);
-                }
-        }
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int q = PIECES - 1; q >= 0; --q) {
+                        mma16816(o[i][j], a0[0], a0[1], b0[0], b0[1], pf[y][i][q]);
+                        mma16816(o[i][j + 1], a1[0], a1[1], b1[0], b1[1], pf[y][i][q]);
+                    }
+            }
     };
 
-    // The places of the groups at hand; the copies, fewer than 32 groups ahead, may already be in the next set.
-    Place now = ahead;
-    int used = 0;
-    for (int q = p; q < hi; q += step, ++used) {
-        if (used % 32 == 0) now = ahead;
-        copy();  // (into the place of the group before this one)
-        cp_wait<D - 1>();
-        Group x;
-        x.at = of_lane(now, used % 32);
-        if (x.at.at < 0) continue;
-        const uint8_t *src = mine + used % D * 32 * HD;
+    auto fetch = [&](Group &x, const Place &place, int i) {  // the warp's group i from its place in the ring
+        x.at = place;
+        const uint8_t *src = mine + i % D * 32 * HD;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < HD / 64; ++i) x.k[n][i] = *reinterpret_cast<const uint4 *>(src + ((n * (HD / 64) + i) * 32 + lane) * 16);
+            for (int j = 0; j < HD / 64; ++j) x.k[n][j] = *reinterpret_cast<const uint4 *>(src + ((n * (HD / 64) + j) * 32 + lane) * 16);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const uint8_t *from = src + 16 * HD + (n * 32 + lane) * VB;
@@ -630,7 +643,39 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 2 : 1) k_kv8_attend(
                 x.v[n][0] = w.x, x.v[n][1] = w.y, x.v[n][2] = w.z, x.v[n][3] = w.w;
             }
         }
-        use(x, q);
+    };
+    // The places of the groups at hand, looked up in sets of 32, of which a turn's groups are of one; the copies, fewer
+    // than 32 groups ahead, may already be in the next set.
+    constexpr int GR = att_groups(HD, NB);
+    Place now = ahead;
+    for (int used = 0; p + used * step < hi; used += GR) {
+        if (used % 32 == 0) now = ahead;
+        // (into the places of the groups of the last turn)
+#pragma unroll
+        for (int y = 0; y < GR; ++y) copy();
+        cp_wait<D - GR>();
+        Group x[GR];
+        Place at[GR];
+        bool all = true;
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+            at[y] = of_lane(now, used % 32 + y);
+            all = all && at[y].at >= 0 && p + (used + y) * step < hi;
+        }
+        const int q = p + used * step;
+        if (all) {
+#pragma unroll
+            for (int y = 0; y < GR; ++y) fetch(x[y], at[y], used + y);
+            use(std::integral_constant<int, GR>{}, x, q);
+        } else {
+#pragma unroll 1
+            for (int y = 0; y < GR; ++y) {
+                const Place one = of_lane(now, used % 32 + y);
+                if (one.at < 0 || q + y * step >= hi) continue;
+                fetch(x[0], one, used + y);
+                use(std::integral_constant<int, 1>{}, x, q + y * step);
+            }
+        }
     }
 
     // the warps' results, joined 64 elements at a time
@@ -867,12 +912,28 @@ int chunk_parts(int64_t units, int64_t span, int64_t slots, int hd) {
     return best;
 }
 
+// Parts of the kernel for few rows: enough for four CTAs an SM, of 128 positions or more.  Measured on a B200 (us): 64
+// sequences of up to 2048 with 148, 296, 444, 592, 1184 CTAs in all 21.8, 19.3, 19.0, 16.8, 21.2; one of 2048 with parts of
+// 128, 256, 512: 6.6, 7.7, 9.1.
+int64_t attend_parts(int64_t units, int64_t span) {
+    if (span < 512) return 1;  // (300 positions: 5.3 us, in two parts 7.1)
+    return std::min<int64_t>({(4 * 148 + units - 1) / units, span / 128, 128});
+}
+
+// Whether the kernel for many rows takes the call.  It starts slower and does more for each byte of the cache: below about
+// 2 million (row, query head, position) of 64 elements the kernel for few rows is faster (B200, us, few / many rows: 1.3 M
+// 14.3 / 14.9 and 16.1 / 17.3, 1.8 M 12.1 / 17.3 and 18.4 / 18.3, 2.2 M 17.0 / 20.6 and 19.0 / 16.0, 2.6 M 22.5 / 16.4,
+// 4.5 M 28.8 / 22.3).  A tile of 128 rows with few of them is no gain: a decoding step stays with the other.
+bool many_rows(const Kv8 &c, int heads, int hd, int window) {
+    const int64_t seen = window > 0 ? std::min<int64_t>(c.cap, (int64_t)window + c.max_new) : c.cap;
+    return (int64_t)c.max_new * (heads / c.kvh) > 32 && (double)c.nrows * heads * (double)seen * (hd / 64) > 2e6;
+}
+
 Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     Cut k{};
     const int group = heads / c.kvh;
     const int64_t rows = (int64_t)c.max_new * group;
-    // rows of one kv head from which on the tensor cores' tiles pay
-    k.chunk = rows > 64;
+    k.chunk = many_rows(c, heads, hd, window);
     const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 && rows > 8 ? 16 : 8;
     k.tile = tile;
     k.tiles = (int)((rows + tile - 1) / tile);
@@ -885,11 +946,10 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
     auto parts = [&](int64_t span) -> int64_t {
         if (k.chunk) return chunk_parts(units, span, (int64_t)c.nrows * heads, hd);
-        // two CTAs an SM; a part is worth its join from 512 positions on
-        int64_t want = std::max<int64_t>(1, std::min<int64_t>({(2 * 148 + units - 1) / units, span / 512, 64}));
-        // a warp sums every 8th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
-        // float32 results are joined from parts of at most 2048 positions
-        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 2047) / 2048);
+        int64_t want = attend_parts(units, span);
+        // a warp sums every 4th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
+        // float32 results are joined from parts of at most 1024 positions
+        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 1023) / 1024);
         return want;
     };
     const int64_t span = span_of(window);
@@ -899,12 +959,14 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     return k;
 }
 
-// The most parts that any window gives: what the workspace has room for.
-int64_t most_parts(const Kv8 &c, int heads, int hd, int type) {
-    const Cut k = attention_cut(c, heads, hd, type, 0);
-    if (k.chunk) return std::min<int64_t>(64, (c.cap + 127) / 128);
-    const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
-    return std::max<int64_t>({1, std::min<int64_t>({(2 * 148 + units - 1) / units, c.cap / 512, 64}), type == LLMB_F32 ? ((int64_t)c.cap + 2047) / 2048 : 1});
+// The most parts that any window gives, by either kernel: what the workspace has room for.
+int64_t most_parts(const Kv8 &c, int heads, int type) {
+    const int64_t rows = (int64_t)c.max_new * (heads / c.kvh), tile = type == LLMB_BF16 && rows > 8 ? 16 : 8;
+    const int64_t units = (int64_t)c.nseq * c.kvh * std::max<int64_t>((rows + tile - 1) / tile, 1);
+    int64_t most = attend_parts(units, c.cap);
+    if (type == LLMB_F32) most = std::max<int64_t>(most, ((int64_t)c.cap + 1023) / 1024);
+    if (rows > 32) most = std::max<int64_t>(most, std::min<int64_t>(64, ((int64_t)c.cap + 127) / 128));
+    return most;
 }
 
 }  // namespace
@@ -963,7 +1025,7 @@ int64_t llmb_kv8_attention_workspace(const llmb_kv8_cache *cache, const llmb_kv8
         return -1;
     }
     int64_t splits = 1;
-    for (int type : {LLMB_F32, LLMB_BF16}) splits = std::max(splits, most_parts(c, heads, cache->head_dim, type));
+    for (int type : {LLMB_F32, LLMB_BF16}) splits = std::max(splits, most_parts(c, heads, type));
     return splits == 1 ? 0 : (int64_t)c.nrows * heads * splits * (8 + 4 * (int64_t)cache->head_dim);
 }
 
