@@ -387,16 +387,16 @@ def _op_check(rc: int) -> None:
         raise LlmError(rc, lib().llmb_last_error(None).decode(errors="replace"))
 
 
-def _ints(t, what: str, shape: tuple) -> int:
-    """The address of a contiguous int32 tensor of that shape."""
-    if _TYPES[t.dtype] != "int32" or t.shape != shape or not t.is_contiguous():
-        _refuse(f"{what} must be a contiguous int32 tensor of shape {shape}")
+def _ints(t, what: str, n: int) -> int:
+    """The address of a contiguous int32 tensor of n elements."""
+    if _TYPES[t.dtype] != "int32" or t.numel() != n or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous int32 tensor of {n} elements")
     return t.data_ptr()
 
 
-def _floats(t, what: str, shape: tuple) -> int:
-    if _TYPES[t.dtype] != F32 or t.shape != shape or not t.is_contiguous():
-        _refuse(f"{what} must be a contiguous float32 tensor of shape {shape}")
+def _floats(t, what: str, n: int) -> int:
+    if _TYPES[t.dtype] != F32 or t.numel() != n or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous float32 tensor of {n} elements")
     return t.data_ptr()
 
 
@@ -407,13 +407,13 @@ class KV8Batch:
     bound the rows and the positions of any one sequence."""
 
     def __init__(self, lens, tables, starts=None, rows: int = 0, max_new: int = 0, max_len: int = 0):
-        if len(tables.shape) != 2 or len(lens.shape) != 1:
-            _refuse("lens must have one dimension, tables two")
+        if len(tables.shape) != 2 or len(lens.shape) != 1 or tables.shape[0] != lens.shape[0]:
+            _refuse("lens must be [n_seq], tables [n_seq, entries]")
         n, entries = lens.shape[0], tables.shape[1]
         self._keep = (lens, tables, starts)
         self.rows = rows
-        self._c = _KV8Batch(_ints(lens, "lens", (n,)), _ints(tables, "tables", (n, entries)),
-                            None if starts is None else _ints(starts, "starts", (n + 1,)),
+        self._c = _KV8Batch(_ints(lens, "lens", n), _ints(tables, "tables", tables.shape[0] * entries),
+                            None if starts is None else _ints(starts, "starts", n + 1),
                             n, entries, rows, max_new, max_len)
         self._ref = C.byref(self._c)
 
@@ -433,7 +433,10 @@ class KV8Cache:
         for x in (k, v):
             if tuple(x.stride())[1:] != (block * hd, hd, 1) or x.stride(0) != k.stride(0):
                 _refuse("k and v must be contiguous within a block and have one block stride")
-        scales = [_floats(x, "a scale", (n, heads)) for x in (k_scale, v_scale)]
+        for x in (k_scale, v_scale):
+            if tuple(x.shape) != (n, heads):
+                _refuse("scales must be [n_blocks, kv_heads]")
+        scales = [_floats(x, "a scale", n * heads) for x in (k_scale, v_scale)]
         self._keep = (k, v, k_scale, v_scale)
         self.kv_heads, self.head_dim = heads, hd
         self._c = _KV8Cache(k.data_ptr(), v.data_ptr(), *scales,
@@ -442,26 +445,30 @@ class KV8Cache:
         self._ref = C.byref(self._c)
         self._lib = lib()
 
-    def _rows(self, batch: KV8Batch, x, what: str, heads: int) -> int:
+    def _rows(self, rows: int, x, what: str, heads: int) -> int:
         """The element distance of the rows of x [rows, heads, head_dim]."""
-        s, hd = x.stride(), self.head_dim
-        if x.shape != (batch.rows, heads, hd) or s[2] != 1 or (s[1] != hd and heads != 1):
-            _refuse(f"{what} must have shape {(batch.rows, heads, hd)} and be contiguous within a row")
-        return s[0] if batch.rows > 1 else max(s[0], heads * hd)
+        hd = self.head_dim
+        if x.shape != (rows, heads, hd):
+            _refuse(f"{what} must have shape {(rows, heads, hd)}")
+        s, s1, s2 = x.stride()
+        if s2 != 1 or (s1 != hd and heads != 1):
+            _refuse(f"{what} must be contiguous within a row")
+        return s if rows > 1 else max(s, heads * hd)
 
-    def _pair(self, batch: KV8Batch, k, v) -> tuple:
+    def _pair(self, rows: int, k, v) -> tuple:
         """(k's address, v's, their type, their row distance); one of them may be None."""
         x = v if k is None else k
         if x is None:
             _refuse("neither k nor v")
-        t, stride = _TYPES[x.dtype], self._rows(batch, x, "k and v", self.kv_heads)
+        dtype = x.dtype
+        t, stride = _TYPES[dtype], self._rows(rows, x, "k and v", self.kv_heads)
         if t not in _ROWS:
             _refuse("rows must be float32, float16 or bfloat16")
         if k is None:
             return None, v.data_ptr(), t, stride
         if v is None:
             return k.data_ptr(), None, t, stride
-        if v.dtype != k.dtype or self._rows(batch, v, "k and v", self.kv_heads) != stride:
+        if v.dtype != dtype or self._rows(rows, v, "k and v", self.kv_heads) != stride:
             _refuse("k and v must have one type and stride")
         return k.data_ptr(), v.data_ptr(), t, stride
 
@@ -469,14 +476,14 @@ class KV8Cache:
         """Writes the rows k, v [rows, kv_heads, head_dim] (llmb_kv8_append)."""
         if k is None or v is None:
             _refuse("append needs k and v")
-        kp, vp, t, stride = self._pair(batch, k, v)
+        kp, vp, t, stride = self._pair(batch.rows, k, v)
         rc = self._lib.llmb_kv8_append(self._ref, batch._ref, kp, vp, t, stride, stream)
         if rc:
             _op_check(rc)
 
     def read(self, batch: KV8Batch, k=None, v=None, stream: int = 0) -> None:
         """Reads what is held at the rows' positions into k, v [rows, kv_heads, head_dim] (llmb_kv8_read)."""
-        kp, vp, t, stride = self._pair(batch, k, v)
+        kp, vp, t, stride = self._pair(batch.rows, k, v)
         rc = self._lib.llmb_kv8_read(self._ref, batch._ref, kp, vp, t, stride, stream)
         if rc:
             _op_check(rc)
@@ -492,12 +499,13 @@ class KV8Cache:
                   stream: int = 0) -> None:
         """Attention of the queries q [rows, heads, head_dim] over the cache into out (llmb_kv8_attention); workspace:
         a contiguous tensor of attention_workspace() bytes."""
-        if len(q.shape) != 3:
+        shape, dtype, rows = q.shape, q.dtype, batch.rows
+        if len(shape) != 3:
             _refuse("q must be [rows, heads, head_dim]")
-        heads, t = q.shape[1], _TYPES[q.dtype]
-        if t not in _ROWS or out.dtype != q.dtype:
+        heads, t = shape[1], _TYPES[dtype]
+        if t not in _ROWS or out.dtype != dtype:
             _refuse("q and out must both be float32, float16 or bfloat16")
-        qs, os_ = self._rows(batch, q, "q", heads), self._rows(batch, out, "out", heads)
+        qs, os_ = self._rows(rows, q, "q", heads), self._rows(rows, out, "out", heads)
         w = n = 0
         if workspace is not None:
             if not workspace.is_contiguous():
@@ -520,49 +528,53 @@ def logits_control(logits, out=None, tokens=None, history=None, history_lens=Non
     if len(shape) != 2:
         _refuse("logits must be [rows, vocab]")
     rows, vocab = shape
-    t, s = _TYPES[dtype], logits.stride()
-    if t not in _ROWS or (s[1] != 1 and vocab != 1):
+    t, (s0, s1) = _TYPES[dtype], logits.stride()
+    if t not in _ROWS or (s1 != 1 and vocab != 1):
         _refuse("logits must be float32, float16 or bfloat16, and contiguous within a row")
-    c = _LogitsCtl()
     op, os_ = None, 0
     if out is not None:
-        o = out.stride()
-        if out.dtype != dtype or out.shape != shape or (o[1] != 1 and vocab != 1):
-            _refuse("out must have the type and shape of logits and be contiguous within a row")
-        op, os_ = out.data_ptr(), o[0] if rows > 1 else max(o[0], vocab)
+        if out.dtype != dtype or out.shape != shape:
+            _refuse("out must have the type and shape of logits")
+        os_, o1 = out.stride()
+        if o1 != 1 and vocab != 1:
+            _refuse("out must be contiguous within a row")
+        op, os_ = out.data_ptr(), os_ if rows > 1 else max(os_, vocab)
+    h = hl = pl = pen = ids = values = starts = bits = None
+    n_hist = n_bias = words = 0
     if history is not None:
-        if len(history.shape) != 2:
+        if len(history.shape) != 2 or history.shape[0] != rows:
             _refuse("history must be [rows, n]")
-        n = history.shape[1]
-        h = _ints(history, "history", (rows, n))
+        n_hist = history.shape[1]
+        h = _ints(history, "history", rows * n_hist)
         if history_lens is not None:
-            history_lens = _ints(history_lens, "history_lens", (rows,))
+            hl = _ints(history_lens, "history_lens", rows)
         if prompt_lens is not None:
-            prompt_lens = _ints(prompt_lens, "prompt_lens", (rows,))
-        if n:  # a history of no tokens is none
-            c.history, c.history_stride, c.history_lens, c.prompt_lens = h, n, history_lens, prompt_lens
+            pl = _ints(prompt_lens, "prompt_lens", rows)
+        if not n_hist:  # a history of no tokens is none
+            h = hl = pl = None
     elif history_lens is not None or prompt_lens is not None:
         _refuse("lengths without a history")
     if penalties is not None:
-        c.penalties = _floats(penalties, "penalties", (rows, 3))
+        pen = _floats(penalties, "penalties", 3 * rows)
     if bias_ids is not None:
-        n = bias_ids.shape[0]
+        n_bias = bias_ids.numel()
         if bias_values is None:
             _refuse("bias_ids without bias_values")
-        ids, values = _ints(bias_ids, "bias_ids", (n,)), _floats(bias_values, "bias_values", (n,))
+        ids, values = _ints(bias_ids, "bias_ids", n_bias), _floats(bias_values, "bias_values", n_bias)
         if bias_starts is not None:
-            bias_starts = _ints(bias_starts, "bias_starts", (rows + 1,))
-        if n:
-            c.n_bias, c.bias_ids, c.bias_values, c.bias_starts = n, ids, values, bias_starts
+            starts = _ints(bias_starts, "bias_starts", rows + 1)
+        if not n_bias:
+            ids = values = starts = None
     elif bias_values is not None or bias_starts is not None:
         _refuse("biases without bias_ids")
     if mask is not None:
-        if len(mask.shape) != 2:
+        if len(mask.shape) != 2 or mask.shape[0] != rows:
             _refuse("mask must be [rows, words]")
-        c.mask_stride = mask.shape[1]
-        c.mask = _ints(mask, "mask", (rows, c.mask_stride))
-    rc = lib().llmb_logits_control(logits.data_ptr(), s[0] if rows > 1 else max(s[0], vocab), t, rows, vocab, c, op, os_,
-                                   None if tokens is None else _ints(tokens, "tokens", (rows,)), stream)
+        words = mask.shape[1]
+        bits = _ints(mask, "mask", rows * words)
+    c = _LogitsCtl(h, hl, pl, n_hist, n_bias, pen, ids, values, starts, bits, words)
+    rc = lib().llmb_logits_control(logits.data_ptr(), s0 if rows > 1 else max(s0, vocab), t, rows, vocab, c, op, os_,
+                                   None if tokens is None else _ints(tokens, "tokens", rows), stream)
     if rc:
         _op_check(rc)
 

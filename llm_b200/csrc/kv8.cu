@@ -113,11 +113,12 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__rest
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
     const int first = max(q.first, 0);
-    const int j = (first >> c.bshift) + blockIdx.x, p0 = j << c.bshift;
-    if (p0 >= q.len) return;
+    const int j = (first >> c.bshift) + blockIdx.x;
     const int b = kv8_block(c, s, j);
     if (b < 0) return;
-    const int lo = max(first - p0, 0), hi = min(q.len - p0, c.block), total = (hi - lo) * PR;
+    const int p0 = j << c.bshift, end = q.first + q.n;
+    if (p0 >= end) return;
+    const int lo = max(first - p0, 0), hi = min(end - p0, c.block), total = (hi - lo) * PR;
     const int64_t row = (int64_t)(q.start + p0 + lo - q.first) * row_stride;
     const int t1 = min((int)(blockIdx.y + 1) * tiles, 2 * c.kvh);
     __shared__ uint32_t red[2][8];
@@ -238,10 +239,10 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
     // blocks counted from the one that holds the first row's position, which may be below 0
-    const int j = (q.first >> c.bshift) + (int)blockIdx.x, p0 = j * c.block;
-    if (p0 >= q.len) return;
+    const int j = (q.first >> c.bshift) + (int)blockIdx.x, p0 = j * c.block, end = q.first + q.n;
+    if (p0 >= end) return;
     const int b = kv8_block(c, s, j);
-    const int lo = max(q.first - p0, 0), hi = min(q.len - p0, c.block);
+    const int lo = max(q.first - p0, 0), hi = min(end - p0, c.block);
     const int64_t row = (int64_t)(q.start + p0 - q.first) * row_stride;
     const int t0 = blockIdx.y * tiles, t1 = min(t0 + tiles, 2 * c.kvh), per = c.block * PR;
     const int shift = c.bshift + (PR == 32 ? 5 : PR == 16 ? 4 : 3);  // of `per`, a power of two
@@ -825,7 +826,7 @@ int kv8_sizes(const char *what, const llmb_kv8_cache *c, const llmb_kv8_batch *b
         return op_error(LLMB_ERR_ARG, "llm: %s: %d sequences, %d table entries, %d rows, max_new %d, max_len %d", what,
                         b->n_seq, b->table_stride, b->n_rows, b->max_new, b->max_len);
     const int64_t held = (int64_t)b->table_stride * c->block;
-    if (held > INT32_MAX - 16384)
+    if (held > kKv8MaxLen)
         return op_error(LLMB_ERR_ARG, "llm: %s: tables of more than 2^31 positions", what);
     k = Kv8{};
     k.bstride = c->block_stride, k.nblocks = c->n_blocks, k.block = c->block, k.kvh = c->kv_heads;
@@ -1048,7 +1049,7 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
     if (c.max_new == 0) return LLMB_OK;
     Kv8Att a{};
     const Cut cut = attention_cut(c, heads, hd, type, window);
-    if ((int64_t)c.kvh * cut.tiles > 65535)
+    if ((int64_t)c.kvh * cut.tiles > 65535 || (int64_t)c.max_new * heads > INT32_MAX)
         return op_error(LLMB_ERR_ARG, "llm: %s: %d rows of a sequence are too many", what, c.max_new);
     const int64_t slots = (int64_t)c.nrows * heads * cut.splits;
     if (cut.splits > 1) {

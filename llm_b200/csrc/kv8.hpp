@@ -10,6 +10,8 @@
 
 namespace llmb {
 
+constexpr int kKv8MaxLen = 0x7fffffff - 16384;  // sums of positions and a block, a step or a set of them stay below 2^31
+
 // The cache and the batch of a call as the kernels take them (include/llm_b200.h describes the fields).
 struct Kv8 {
     uint8_t *k, *v;
@@ -20,7 +22,8 @@ struct Kv8 {
     int nseq, tstride, nrows, max_new, cap;  // cap: the most positions a sequence can have here
 };
 
-// A sequence's share of the call: rows start .. start + n - 1 are its positions first .. first + n - 1 = len - 1.
+// A sequence's share of the call: rows start .. start + n - 1 are its positions first .. first + n - 1 (below 0 for the
+// first rows of one that has more rows than positions: they have none); it sees positions below len.
 struct Kv8Seq {
     int start, n, len, first;
 };
@@ -36,10 +39,11 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8 &c, int s) {
         const int per = c.nrows / c.nseq;
         a = s * per, b = a + per;
     }
+    const int len = min(max(__ldg(c.lens + s), 0), kKv8MaxLen);
     q.start = a;
     q.n = min(b - a, c.max_new);
-    q.len = min(max(__ldg(c.lens + s), 0), c.cap);
-    q.first = q.len - q.n;  // below 0 where a sequence has more rows than positions: the first rows have none
+    q.len = min(len, c.cap);
+    q.first = len - (b - a);
     return q;
 }
 

@@ -585,6 +585,37 @@ def test_captured_steps_on_another_stream():
 
 
 @gpu
+def test_bounds_that_are_too_small_shift_nothing():
+    """max_new and max_len below what a sequence has: its first rows are taken, at their own positions, and positions
+    past max_len are not seen."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(14)
+    d = _filled(2, 16, 64, "int8", [100], rng)
+    k, v = (_rows(torch, rng, 20, 2, 64, "f32") for _ in range(2))
+    batch = KV8Batch(torch.tensor([100], dtype=torch.int32).cuda(), d.dtables, torch.tensor([0, 20], dtype=torch.int32).cuda(),
+                     rows=20, max_new=7, max_len=60)
+    d.cache.append(batch, k, v)  # positions 80..86
+    d.plain.append(d.tables[0], 87, torch.stack([k[:7], v[:7]]).cpu())
+    d.same_as_plain([87])
+    out = torch.full((20, 2, 64), 5.0, device="cuda")
+    d.cache.read(batch, out)
+    assert torch.equal(out[:7].cpu(), d.plain.rows(d.tables[0], 87, 7)[0]) and (out[7:] == 5).all()
+    q = _rows(torch, rng, 20, 4, 64, "f32")
+    got, want = torch.full_like(q, 5.0), torch.full((7, 4, 64), 5.0, device="cuda")
+    d.cache.attention(batch, q, got, workspace=_workspace(d, batch, 4))
+    one = KV8Batch(torch.tensor([60], dtype=torch.int32).cuda(), d.dtables, rows=1)
+    for r in range(7):  # each of the rows sees positions 0..59
+        d.cache.attention(one, q[r:r + 1], want[r:r + 1], workspace=_workspace(d, one, 4))
+    # (the two batches may cut the positions into parts differently: two results within their tolerance)
+    _, size = _reference(d, [60], [1], q[:1].cpu(), 0.125, 0)
+    tol = 2 * _tolerance(size.expand(7, 2).clone(), 60, 64, "f32", want.cpu().double())
+    s = torch.einsum("rhd,rhd->rh", q[:7].cpu().double().abs(), torch.ones(7, 4, 64, dtype=torch.float64)).max()
+    big = 0.125 * s * d.plain.rows(d.tables[0], 60, 60).abs().max().double()  # scale sum |q| max |k| bounds every row's S
+    tol = tol.maximum(2 * _tolerance(torch.stack([big, size[0, 1]]).expand(7, 2).clone(), 60, 64, "f32", want.cpu().double()))
+    assert ((got[:7] - want).abs().cpu().double() <= tol).all() and (got[7:] == 5).all()
+
+
+@gpu
 def test_refusals_on_the_device():
     """Host memory, a missing workspace, and no rows."""
     torch, _, _ = _t()
