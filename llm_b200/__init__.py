@@ -18,6 +18,7 @@ not been built (``python -m llm_b200.build``).
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import os
 from dataclasses import dataclass
 
@@ -359,23 +360,21 @@ class GPU:
 # device current, until the work is done. stream is a cudaStream_t handle
 # (torch.cuda.current_stream().cuda_stream), 0 the default stream.
 #
-# A decoding step's kernels take a few microseconds, so these wrappers check
-# with plain comparisons and build a message only for what they refuse.
+# Their checks and calls are in csrc/call.c.
 
-_NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": "int8", "float8_e4m3fn": "e4m3", "int32": "int32",
-          "uint32": "int32"}
-_ROWS = (F32, F16, BF16)
+_NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": 10, "float8_e4m3fn": 11, "int32": 20, "uint32": 20}
 
 
 class _Types(dict):
-    """dtype -> its entry in _NAMES, or None."""
+    """dtype -> its entry in _NAMES, or -1."""
 
     def __missing__(self, dtype):
-        self[dtype] = t = _NAMES.get(str(dtype).rsplit(".", 1)[-1])
+        self[dtype] = t = _NAMES.get(str(dtype).rsplit(".", 1)[-1], -1)
         return t
 
 
 _TYPES = _Types()
+_native_calls = None
 
 
 def _refuse(msg: str):
@@ -387,16 +386,24 @@ def _op_check(rc: int) -> None:
         raise LlmError(rc, lib().llmb_last_error(None).decode(errors="replace"))
 
 
-def _ints(t, what: str, n: int) -> int:
-    """The address of a contiguous int32 tensor of n elements."""
-    if _TYPES[t.dtype] != "int32" or t.numel() != n or not t.is_contiguous():
-        _refuse(f"{what} must be a contiguous int32 tensor of {n} elements")
-    return t.data_ptr()
+def _calls():
+    """The native calls, with the library they are linked to."""
+    global _native_calls
+    if _native_calls is None:
+        lib()  # says how to build where it is missing
+        try:
+            module = importlib.import_module("._native", __name__)
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -m llm_b200.build`") from e
+        module.setup(_TYPES, _refuse, _op_check)
+        _native_calls = module
+    return _native_calls
 
 
-def _floats(t, what: str, n: int) -> int:
-    if _TYPES[t.dtype] != F32 or t.numel() != n or not t.is_contiguous():
-        _refuse(f"{what} must be a contiguous float32 tensor of {n} elements")
+def _flat(t, what: str, name: str, shape: tuple) -> int:
+    """The address of a contiguous tensor of that type and shape."""
+    if _TYPES[t.dtype] != _NAMES[name] or tuple(t.shape) != shape or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous {name} tensor of shape {shape}")
     return t.data_ptr()
 
 
@@ -412,10 +419,10 @@ class KV8Batch:
         n, entries = lens.shape[0], tables.shape[1]
         self._keep = (lens, tables, starts)
         self.rows = rows
-        self._c = _KV8Batch(_ints(lens, "lens", n), _ints(tables, "tables", tables.shape[0] * entries),
-                            None if starts is None else _ints(starts, "starts", n + 1),
+        self._c = _KV8Batch(_flat(lens, "lens", "int32", (n,)), _flat(tables, "tables", "int32", (n, entries)),
+                            None if starts is None else _flat(starts, "starts", "int32", (n + 1,)),
                             n, entries, rows, max_new, max_len)
-        self._ref = C.byref(self._c)
+        self._at = C.addressof(self._c)
 
 
 class KV8Cache:
@@ -428,69 +435,31 @@ class KV8Cache:
             _refuse("k and v must be [n_blocks, kv_heads, block, head_dim]")
         n, heads, block, hd = k.shape
         t = _TYPES[k.dtype]
-        if t not in ("int8", "e4m3") or t != _TYPES[v.dtype]:
+        if t not in (10, 11) or t != _TYPES[v.dtype]:
             _refuse("k and v must both be int8 or both float8_e4m3fn")
         for x in (k, v):
             if tuple(x.stride())[1:] != (block * hd, hd, 1) or x.stride(0) != k.stride(0):
                 _refuse("k and v must be contiguous within a block and have one block stride")
-        for x in (k_scale, v_scale):
-            if tuple(x.shape) != (n, heads):
-                _refuse("scales must be [n_blocks, kv_heads]")
-        scales = [_floats(x, "a scale", n * heads) for x in (k_scale, v_scale)]
+        scales = [_flat(x, "a scale", "float32", (n, heads)) for x in (k_scale, v_scale)]
         self._keep = (k, v, k_scale, v_scale)
         self.kv_heads, self.head_dim = heads, hd
         self._c = _KV8Cache(k.data_ptr(), v.data_ptr(), *scales,
                             max(k.stride(0), heads * block * hd) if n == 1 else k.stride(0), n, block, heads, hd,
-                            KV8_INT8 if t == "int8" else KV8_E4M3)
-        self._ref = C.byref(self._c)
-        self._lib = lib()
-
-    def _rows(self, rows: int, x, what: str, heads: int) -> int:
-        """The element distance of the rows of x [rows, heads, head_dim]."""
-        hd = self.head_dim
-        if x.shape != (rows, heads, hd):
-            _refuse(f"{what} must have shape {(rows, heads, hd)}")
-        s, s1, s2 = x.stride()
-        if s2 != 1 or (s1 != hd and heads != 1):
-            _refuse(f"{what} must be contiguous within a row")
-        return s if rows > 1 else max(s, heads * hd)
-
-    def _pair(self, rows: int, k, v) -> tuple:
-        """(k's address, v's, their type, their row distance); one of them may be None."""
-        x = v if k is None else k
-        if x is None:
-            _refuse("neither k nor v")
-        dtype = x.dtype
-        t, stride = _TYPES[dtype], self._rows(rows, x, "k and v", self.kv_heads)
-        if t not in _ROWS:
-            _refuse("rows must be float32, float16 or bfloat16")
-        if k is None:
-            return None, v.data_ptr(), t, stride
-        if v is None:
-            return k.data_ptr(), None, t, stride
-        if v.dtype != dtype or self._rows(rows, v, "k and v", self.kv_heads) != stride:
-            _refuse("k and v must have one type and stride")
-        return k.data_ptr(), v.data_ptr(), t, stride
+                            KV8_INT8 if t == 10 else KV8_E4M3)
+        self._at = C.addressof(self._c)
+        self._rows, self._attend = _calls().rows, _calls().attention
 
     def append(self, batch: KV8Batch, k, v, stream: int = 0) -> None:
         """Writes the rows k, v [rows, kv_heads, head_dim] (llmb_kv8_append)."""
-        if k is None or v is None:
-            _refuse("append needs k and v")
-        kp, vp, t, stride = self._pair(batch.rows, k, v)
-        rc = self._lib.llmb_kv8_append(self._ref, batch._ref, kp, vp, t, stride, stream)
-        if rc:
-            _op_check(rc)
+        self._rows(0, self._at, batch._at, batch.rows, self.kv_heads, self.head_dim, k, v, stream)
 
     def read(self, batch: KV8Batch, k=None, v=None, stream: int = 0) -> None:
         """Reads what is held at the rows' positions into k, v [rows, kv_heads, head_dim] (llmb_kv8_read)."""
-        kp, vp, t, stride = self._pair(batch.rows, k, v)
-        rc = self._lib.llmb_kv8_read(self._ref, batch._ref, kp, vp, t, stride, stream)
-        if rc:
-            _op_check(rc)
+        self._rows(1, self._at, batch._at, batch.rows, self.kv_heads, self.head_dim, k, v, stream)
 
     def attention_workspace(self, batch: KV8Batch, heads: int) -> int:
         """Bytes of workspace for attention() with that many query heads (llmb_kv8_attention_workspace)."""
-        n = self._lib.llmb_kv8_attention_workspace(self._ref, batch._ref, heads)
+        n = lib().llmb_kv8_attention_workspace(C.byref(self._c), C.byref(batch._c), heads)
         if n < 0:
             _op_check(ERR_ARG)
         return n
@@ -499,22 +468,7 @@ class KV8Cache:
                   stream: int = 0) -> None:
         """Attention of the queries q [rows, heads, head_dim] over the cache into out (llmb_kv8_attention); workspace:
         a contiguous tensor of attention_workspace() bytes."""
-        shape, dtype, rows = q.shape, q.dtype, batch.rows
-        if len(shape) != 3:
-            _refuse("q must be [rows, heads, head_dim]")
-        heads, t = shape[1], _TYPES[dtype]
-        if t not in _ROWS or out.dtype != dtype:
-            _refuse("q and out must both be float32, float16 or bfloat16")
-        qs, os_ = self._rows(rows, q, "q", heads), self._rows(rows, out, "out", heads)
-        w = n = 0
-        if workspace is not None:
-            if not workspace.is_contiguous():
-                _refuse("workspace must be contiguous")
-            w, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        rc = self._lib.llmb_kv8_attention(self._ref, batch._ref, q.data_ptr(), qs, out.data_ptr(), os_, t, heads, scale,
-                                          window, w or None, n, stream)
-        if rc:
-            _op_check(rc)
+        self._attend(self._at, batch._at, batch.rows, self.head_dim, q, out, scale, window, workspace, stream)
 
 
 def logits_control(logits, out=None, tokens=None, history=None, history_lens=None, prompt_lens=None, penalties=None,
@@ -524,59 +478,8 @@ def logits_control(logits, out=None, tokens=None, history=None, history_lens=Non
     history_lens, prompt_lens [rows] int32; penalties [rows, 3] float32 (repetition, presence, frequency); bias_ids
     int32 and bias_values float32 [n], with bias_starts [rows + 1] int32 for biases of each row's own; mask
     [rows, ceil(vocab / 32)] int32, bit 1 where a token is allowed."""
-    shape, dtype = logits.shape, logits.dtype
-    if len(shape) != 2:
-        _refuse("logits must be [rows, vocab]")
-    rows, vocab = shape
-    t, (s0, s1) = _TYPES[dtype], logits.stride()
-    if t not in _ROWS or (s1 != 1 and vocab != 1):
-        _refuse("logits must be float32, float16 or bfloat16, and contiguous within a row")
-    op, os_ = None, 0
-    if out is not None:
-        if out.dtype != dtype or out.shape != shape:
-            _refuse("out must have the type and shape of logits")
-        os_, o1 = out.stride()
-        if o1 != 1 and vocab != 1:
-            _refuse("out must be contiguous within a row")
-        op, os_ = out.data_ptr(), os_ if rows > 1 else max(os_, vocab)
-    h = hl = pl = pen = ids = values = starts = bits = None
-    n_hist = n_bias = words = 0
-    if history is not None:
-        if len(history.shape) != 2 or history.shape[0] != rows:
-            _refuse("history must be [rows, n]")
-        n_hist = history.shape[1]
-        h = _ints(history, "history", rows * n_hist)
-        if history_lens is not None:
-            hl = _ints(history_lens, "history_lens", rows)
-        if prompt_lens is not None:
-            pl = _ints(prompt_lens, "prompt_lens", rows)
-        if not n_hist:  # a history of no tokens is none
-            h = hl = pl = None
-    elif history_lens is not None or prompt_lens is not None:
-        _refuse("lengths without a history")
-    if penalties is not None:
-        pen = _floats(penalties, "penalties", 3 * rows)
-    if bias_ids is not None:
-        n_bias = bias_ids.numel()
-        if bias_values is None:
-            _refuse("bias_ids without bias_values")
-        ids, values = _ints(bias_ids, "bias_ids", n_bias), _floats(bias_values, "bias_values", n_bias)
-        if bias_starts is not None:
-            starts = _ints(bias_starts, "bias_starts", rows + 1)
-        if not n_bias:
-            ids = values = starts = None
-    elif bias_values is not None or bias_starts is not None:
-        _refuse("biases without bias_ids")
-    if mask is not None:
-        if len(mask.shape) != 2 or mask.shape[0] != rows:
-            _refuse("mask must be [rows, words]")
-        words = mask.shape[1]
-        bits = _ints(mask, "mask", rows * words)
-    c = _LogitsCtl(h, hl, pl, n_hist, n_bias, pen, ids, values, starts, bits, words)
-    rc = lib().llmb_logits_control(logits.data_ptr(), s0 if rows > 1 else max(s0, vocab), t, rows, vocab, c, op, os_,
-                                   None if tokens is None else _ints(tokens, "tokens", rows), stream)
-    if rc:
-        _op_check(rc)
+    _calls().logits(logits, out, tokens, history, history_lens, prompt_lens, penalties, bias_ids, bias_values, bias_starts,
+                   mask, stream)
 
 
 def NewGPU(path: str, ctx: int = 0, device: int = 0) -> GPU:

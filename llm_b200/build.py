@@ -1,4 +1,5 @@
-"""Builds llm_b200/libllmb200.so with nvcc for sm_100a (in-tree, so it travels with the repository).
+"""Builds llm_b200/libllmb200.so with nvcc for sm_100a, and _native.abi3.so, the Python calls of its operators (in-tree, so
+that they travel with the repository).
 
     python -m llm_b200.build          # incremental
     python -m llm_b200.build --force  # rebuild everything
@@ -9,12 +10,14 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllmb200.so")
+CALL = os.path.join(HERE, "_native.abi3.so")
 SOURCES = ["gguf.cpp", "kernels.cu", "gemm.cu", "decode.cu", "engine.cu", "noalloc.cu", "ops.cpp", "kv8.cu", "kv8_chunk.cu", "logits.cu"]
 HEADERS = ["gguf.hpp", "device.hpp", "kernels.hpp", "ops.hpp", "kv8.hpp", "kv8_chunk.hpp", os.path.join("..", "..", "include", "llm_b200.h")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -50,6 +53,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
         subprocess.run([_nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-lcudart_static", "-lrt", "-ldl", "-lpthread"],
                        check=True)
         os.replace(tmp, LIB)
+    src = os.path.join(CSRC, "call.c")
+    header = os.path.join(ROOT, "include", "llm_b200.h")
+    if force or not os.path.exists(CALL) or os.path.getmtime(CALL) < max(os.path.getmtime(f) for f in (src, header, __file__)):
+        tmp = CALL + ".tmp"
+        subprocess.run([os.environ.get("CC", "gcc"), "-O2", "-std=c11", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
+                        "-I", sysconfig.get_paths()["include"], src, "-o", tmp, "-L", HERE, "-l:libllmb200.so",
+                        "-Wl,-rpath,$ORIGIN"], check=True)
+        os.replace(tmp, CALL)
     return LIB
 
 

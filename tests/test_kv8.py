@@ -98,7 +98,14 @@ def test_python_checks_refuse_wrong_tensors():
             cache.append(batch, *a)
     with pytest.raises(LlmError):
         cache.read(batch)
+    for a in ((1, 2), ("k", x), (x, object())):  # no tensors at all
+        with pytest.raises((AttributeError, TypeError)):
+            cache.append(batch, *a)
+    with pytest.raises(TypeError):
+        cache.append(batch, x, x, stream="0")
     q = torch.zeros(2, 4, 64)
+    with pytest.raises(LlmError, match="window"):
+        cache.attention(batch, q, q, window=1 << 40)
     for a in ((q, q.half()), (q, q[:1]), (q[0], q[0]), (q.transpose(0, 1), q)):
         with pytest.raises(LlmError):
             cache.attention(batch, *a)
