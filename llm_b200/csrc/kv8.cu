@@ -916,25 +916,29 @@ int chunk_parts(int64_t units, int64_t span, int64_t slots, int hd) {
 // Parts of the kernel for few rows: enough for four CTAs an SM, of 128 positions or more.  Measured on a B200 (us): 64
 // sequences of up to 2048 with 148, 296, 444, 592, 1184 CTAs in all 21.8, 19.3, 19.0, 16.8, 21.2; one of 2048 with parts of
 // 128, 256, 512: 6.6, 7.7, 9.1.
-int64_t attend_parts(int64_t units, int64_t span) {
+int64_t attend_parts(const Kv8 &c, int64_t units, int64_t span) {
     if (span < 512) return 1;  // (300 positions: 5.3 us, in two parts 7.1)
-    return std::min<int64_t>({(4 * 148 + units - 1) / units, span / 128, 128});
+    // (one token of sequences of any lengths: rather more than a wave; a chunk's tiles are alike: rather less)
+    const int64_t fill = c.max_new > 1 ? std::max<int64_t>(4 * 148 / units, 1) : (4 * 148 + units - 1) / units;
+    return std::min<int64_t>({fill, span / 128, 128});
 }
 
 // Whether the kernel for many rows takes the call.  It starts slower and does more for each byte of the cache: below about
-// 2 million (row, query head, position) of 64 elements the kernel for few rows is faster (B200, us, few / many rows: 1.3 M
-// 14.3 / 14.9 and 16.1 / 17.3, 1.8 M 12.1 / 17.3 and 18.4 / 18.3, 2.2 M 17.0 / 20.6 and 19.0 / 16.0, 2.6 M 22.5 / 16.4,
-// 4.5 M 28.8 / 22.3).  A tile of 128 rows with few of them is no gain: a decoding step stays with the other.
-bool many_rows(const Kv8 &c, int heads, int hd, int window) {
+// 2 million (row, query head, position) of 64 elements the kernel for few rows is faster, 2.5 million where rows are two
+// pieces and its tiles 8 rows (B200, us, few / many rows; bfloat16: 1.3 M 14.5 / 16.5, 1.8 M 15.9 / 15.6, 2.2 M 19.0 / 15.3;
+// float32: 1.8 M 16.2 / 17.0, 2.2 M 16.5 / 17.7 and 17.0 / 21.3, 2.6 M 24.1 / 19.6).  A tile of 128 rows with few of them
+// is no gain: a decoding step stays with the other.
+bool many_rows(const Kv8 &c, int heads, int hd, int type, int window) {
     const int64_t seen = window > 0 ? std::min<int64_t>(c.cap, (int64_t)window + c.max_new) : c.cap;
-    return (int64_t)c.max_new * (heads / c.kvh) > 32 && (double)c.nrows * heads * (double)seen * (hd / 64) > 2e6;
+    return (int64_t)c.max_new * (heads / c.kvh) > 32 &&
+           (double)c.nrows * heads * (double)seen * (hd / 64) > (type == LLMB_BF16 ? 2e6 : 2.5e6);
 }
 
 Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     Cut k{};
     const int group = heads / c.kvh;
     const int64_t rows = (int64_t)c.max_new * group;
-    k.chunk = many_rows(c, heads, hd, window);
+    k.chunk = many_rows(c, heads, hd, type, window);
     const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 && rows > 8 ? 16 : 8;
     k.tile = tile;
     k.tiles = (int)((rows + tile - 1) / tile);
@@ -947,7 +951,7 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
     auto parts = [&](int64_t span) -> int64_t {
         if (k.chunk) return chunk_parts(units, span, (int64_t)c.nrows * heads, hd);
-        int64_t want = attend_parts(units, span);
+        int64_t want = attend_parts(c, units, span);
         // a warp sums every 4th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
         // float32 results are joined from parts of at most 1024 positions
         if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 1023) / 1024);
@@ -964,7 +968,7 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
 int64_t most_parts(const Kv8 &c, int heads, int type) {
     const int64_t rows = (int64_t)c.max_new * (heads / c.kvh), tile = type == LLMB_BF16 && rows > 8 ? 16 : 8;
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max<int64_t>((rows + tile - 1) / tile, 1);
-    int64_t most = attend_parts(units, c.cap);
+    int64_t most = attend_parts(c, units, c.cap);
     if (type == LLMB_F32) most = std::max<int64_t>(most, ((int64_t)c.cap + 1023) / 1024);
     if (rows > 32) most = std::max<int64_t>(most, std::min<int64_t>(64, ((int64_t)c.cap + 127) / 128));
     return most;

@@ -251,12 +251,17 @@ __device__ __forceinline__ void load_queries(const Kv8Att &a, const Kv8Seq &sq, 
                                              int lane, uint8_t *q_smem, float *fac, float unit) {
     constexpr int PN = HD / 64, QP = kQPieces<T>, V4 = (int)sizeof(T) / 2, B = sizeof(T) == 4 && HD == 128 ? 4 : 8;
     const int sub = lane & 7;
+    // row warp * 32 + lane / 8 and every fourth after it: token and head in its group, without more divisions
+    int tok = (row0 + warp * 32 + (lane >> 3)) / a.group, in = row0 + warp * 32 + (lane >> 3) - tok * a.group;
+    const int tok4 = 4 / a.group, in4 = 4 - tok4 * a.group;
     for (int it0 = 0; it0 < 8; it0 += B) {  // B rows' loads in flight
         uint4 raw[B][PN][V4];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            const int r = row0 + warp * 32 + (it0 + i) * 4 + (lane >> 3), tok = r / a.group, h = head * a.group + r - tok * a.group;
-            const T *src = static_cast<const T *>(a.q) + (int64_t)(sq.start + tok) * a.q_stride + h * HD + 8 * sub;
+            const int r = row0 + warp * 32 + (it0 + i) * 4 + (lane >> 3);
+            const T *src = static_cast<const T *>(a.q) + (int64_t)(sq.start + tok) * a.q_stride + (head * a.group + in) * HD + 8 * sub;
+            tok += tok4, in += in4;
+            if (in >= a.group) in -= a.group, ++tok;
 #pragma unroll
             for (int p = 0; p < PN; ++p)
 #pragma unroll
@@ -472,42 +477,57 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
             if (ok && steps > 0) ok = bar_wait(&bar.o[w], 0, fail);
             fence_after();
             ok = __all_sync(kFull, ok);
-            // the row's result
-            const int64_t at = ((int64_t)(sq.start + tok) * a.heads + h) * a.splits + blockIdx.x;
-            const float inv = a.splits == 1 ? (l == 0.f ? 0.f : unit / l) : unit;
-            if (on && a.splits > 1) a.part_ml[at] = make_float2(m, ok ? l : NAN);
+            // The rows' results, CW columns at a time by way of the tile's queries' place (their products are done), so that
+            // lanes store neighbouring elements: a lane for each row would touch 32 lines an instruction (3.5 K cycles).
+            constexpr int CW = L::q_tile >= 4 * 32 * (32 + 4) * 4 ? 32 : 16, PITCH = CW + 4, LR = CW / 4;  // lanes of a row
+            static_assert(L::q_tile >= 4 * 32 * PITCH * 4, "the results' place");
+            float *stage = reinterpret_cast<float *>(smem + w * L::q_tile) + wq * 32 * PITCH;
+            const int64_t part = ((int64_t)(sq.start + tok) * a.heads + h) * a.splits + blockIdx.x;
+            const bool split = a.splits > 1;
+            // where the lane's row goes (-1: nowhere), and the rows that it stores pieces of
+            const int64_t own = !on ? -1 : split ? part * HD : (int64_t)(sq.start + tok) * a.out_stride + h * HD;
+            const float inv = split ? unit : l == 0.f ? 0.f : unit / l;
+            if (on && split) a.part_ml[part] = make_float2(m, ok ? l : NAN);
 #pragma unroll 1
-            for (int k = 0; k < HD / 32; ++k) {
-                uint32_t x[32];
-                if (steps > 0 && ok) {
-                    tm_ld32(am + 32 * k, x);
-                    tm_wait(x);
-                    if (SUM > 0 && steps > SUM) {
-                        uint32_t r[32];
-                        tm_ld32(om + 32 * k, r);
-                        tm_wait(r);
+            for (int k = 0; k < HD / CW; ++k) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(r[e]));
+                for (int k2 = 0; k2 < CW; k2 += 16) {
+                    uint32_t x[16];
+                    if (steps > 0 && ok) {
+                        tm_ld16(am + CW * k + k2, x);
+                        tm_wait(x);
+                        if (SUM > 0 && steps > SUM) {
+                            uint32_t r2[16];
+                            tm_ld16(om + CW * k + k2, r2);
+                            tm_wait(r2);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(r2[e]));
+                        }
                     }
-                } else {
+                    float y[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(ok ? 0.f : NAN);
+                    for (int e = 0; e < 16; ++e) y[e] = !ok ? NAN : steps == 0 || (!split && l == 0.f) ? 0.f : __uint_as_float(x[e]) * inv;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4 *>(stage + lane * PITCH + k2 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
                 }
-                if (on && a.splits > 1) {
-                    float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * HD + 32 * k);
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        dst[e] = make_float4(__uint_as_float(x[4 * e]) * inv, __uint_as_float(x[4 * e + 1]) * inv,
-                                             __uint_as_float(x[4 * e + 2]) * inv, __uint_as_float(x[4 * e + 3]) * inv);
-                } else if (on) {
-                    T *dst = static_cast<T *>(a.out) + (int64_t)(sq.start + tok) * a.out_stride + h * HD + 32 * k;
-                    constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll
-                    for (int e = 0; e < 32; e += E) {
-                        T v[E];
-#pragma unroll
-                        for (int i = 0; i < E; ++i) v[i] = kv8_from<T>(l == 0.f && ok ? 0.f : __uint_as_float(x[e + i]) * inv);
-                        *reinterpret_cast<uint4 *>(dst + e) = *reinterpret_cast<const uint4 *>(v);
+                for (int i = 0; i < LR; ++i) {
+                    const int row = i * (32 / LR) + lane / LR, c4 = lane % LR * 4;
+                    const int64_t to = __shfl_sync(kFull, own, row);
+                    const float4 v = *reinterpret_cast<const float4 *>(stage + row * PITCH + c4);
+                    if (to < 0) continue;
+                    if (split) {
+                        *reinterpret_cast<float4 *>(a.part_o + to + CW * k + c4) = v;
+                    } else {
+                        T *dst = static_cast<T *>(a.out) + to + CW * k + c4;
+                        if constexpr (sizeof(T) == 4) {
+                            *reinterpret_cast<float4 *>(dst) = v;
+                        } else {
+                            const T o[4] = {kv8_from<T>(v.x), kv8_from<T>(v.y), kv8_from<T>(v.z), kv8_from<T>(v.w)};
+                            *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
+                        }
                     }
                 }
                 __syncwarp();
