@@ -18,8 +18,9 @@
 //              weights P over S as float16.
 //
 // While the softmax of one tile runs, the tensor cores work on the other.
-// The accumulators are rescaled only when a row's maximum grows by more than
-// 2^8, which is rare after the first positions.
+// The accumulators are rescaled only when a weight would come out above 2^14,
+// which is rare after the first positions (bfloat16 rows do not even look for
+// a step's maximum otherwise).
 //
 // Precision is that of the kernel for few rows (kv8.cu): float32 queries and
 // weights are two float16 pieces each, float16 queries one and their weights
@@ -324,11 +325,13 @@ __device__ __forceinline__ float row_top(const uint32_t (&x)[4][32], const Group
     return top;
 }
 
-// A row's weights 2^(score + shift) into tensor memory over its scores; returns their sum without V's scales.
+// A row's weights 2^(score + shift) into tensor memory over its scores; returns their sum without V's scales. big becomes
+// the largest sum of 16 of them: none of them is larger (NaN stays NaN).
 template <int PP, bool WHOLE>
 __device__ __forceinline__ float row_weights(const uint32_t (&x)[4][32], uint32_t sm, const Group *gp, float fac, float shift,
-                                             int b0, int b1) {
+                                             int b0, int b1, float &big) {
     float l = 0.f;
+    big = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         uint32_t ph[16], pl[16];
@@ -356,7 +359,9 @@ __device__ __forceinline__ float row_weights(const uint32_t (&x)[4][32], uint32_
                     pl[8 * g + e / 2] = pack_half2(y0 - b.x, y1 - b.y);
                 }
             }
-            l = fmaf(unpack2(sum2).x + unpack2(sum2).y, gr.unlv, l);
+            const float sum = unpack2(sum2).x + unpack2(sum2).y;
+            big = sum <= big ? big : sum;
+            l = fmaf(sum, gr.unlv, l);
         }
         // 32 columns for 32 positions: 16 of first pieces, 16 of second ones
         tm_st16(sm + 32 * k, ph);
@@ -438,18 +443,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 for (int k = 0; k < 4; ++k) tm_ld32(sm + 32 * k, x[k]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tm_wait(x[k]);
-                const float top = whole ? row_top<true>(x, gp, fac, b0, b1) : row_top<false>(x, gp, fac, b0, b1);
-                // (every product issued before this step's S is done)
-                const bool add = SUM > 0 && j > 0 && j % SUM1 == 0;
-                float f = 1.f;
-                const bool grow = __any_sync(kFull, top - m > 8.f);
-                if (grow) {
+                auto weigh = [&](float &big) {
+                    return whole ? row_weights<PP, true>(x, sm, gp, fac, 6.f - m, b0, b1, big)
+                                 : row_weights<PP, false>(x, sm, gp, fac, 6.f - m, b0, b1, big);
+                };
+                auto find = [&]() { return whole ? row_top<true>(x, gp, fac, b0, b1) : row_top<false>(x, gp, fac, b0, b1); };
+                float f = 1.f, big, sum = 0.f;
+                bool fresh;
+                auto raise = [&](float top) {
                     const float n = fmaxf(top, m);
                     f = kv8_exp2(m - n);
                     m = n;
                     l *= f;
+                };
+                if constexpr (PP == 1) {
+                    // The maximum of the steps before serves as long as no weight is above 2^14 (float16 ends at 2^16);
+                    // looking for this step's first took a fifth of the time.
+                    fresh = j == 0;
+                    if (!fresh) {
+                        sum = weigh(big);
+                        fresh = __any_sync(kFull, !(big <= 16384.f));
+                    }
+                    if (fresh) {
+                        raise(find());
+                        sum = weigh(big);
+                    }
+                } else {  // (two pieces leave no registers for weighing twice: 232 us for 194)
+                    const float top = find();
+                    fresh = __any_sync(kFull, top - m > 8.f);
+                    if (fresh) raise(top);
+                    sum = weigh(big);
                 }
-                if (j > 0 && (grow || add)) {
+                l += sum;
+                // (every product issued before this step's S is done)
+                const bool add = SUM > 0 && j > 0 && j % SUM1 == 0;
+                if (j > 0 && (fresh || add)) {
 #pragma unroll 1
                     for (int k = 0; k < HD; k += 16) {
                         uint32_t r[16], v[16];
@@ -468,7 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                         if (!add) tm_st16(am + k, v);
                     }
                 }
-                l += whole ? row_weights<PP, true>(x, sm, gp, fac, 6.f - m, b0, b1) : row_weights<PP, false>(x, sm, gp, fac, 6.f - m, b0, b1);
                 tm_st_wait();
                 fence_before();
                 __syncwarp();
