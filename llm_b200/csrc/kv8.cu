@@ -103,8 +103,11 @@ __device__ __forceinline__ void kv8_unpack(const uint4 &r, float (&x)[16 / sizeo
 // head after the other): a tile's new rows are held in registers (U pieces of
 // 16 bytes a thread) between the maximum and the rounding, so they are read
 // once, and the next tile's are on their way meanwhile.  Bound by the memory's
-// rate; several tiles a block of threads spread the three look-ups (lengths,
-// table, scale) that come before the first load.
+// rate (64 bfloat16 prompts of up to 1000 positions, 16 tiles of 64 x 128: 202
+// MB in 44 us, 70 % of the measured copy rate; with one tile a block of
+// threads, whose three look-ups, lengths, table and scale, come before its
+// first load, and a conversion a value 65 us).  A decoding step is 2 us, a
+// launch's latency.
 template <class T, bool E4M3, int HD, int U>
 __global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__restrict__ k, const T *__restrict__ v,
                                                     int64_t row_stride, int tiles) {
@@ -230,7 +233,9 @@ void append_launch(const Kv8 &c, const void *k, const void *v, int64_t row_strid
 // --------------------------------------------------------------- read --
 
 // One block of a sequence and `tiles` of its 2 kv_heads tiles, 16 bytes of
-// result a thread and step, four steps' loads in flight.
+// result a thread and step, four steps' loads in flight.  Bound by the
+// memory's rate: 352 MB, two thirds of them written, in 74 us, 73 % of the
+// measured copy rate (eight steps in flight: the same).
 template <class T, bool E4M3, int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k, T *__restrict__ v,
                                                   int64_t row_stride, int tiles) {
@@ -334,6 +339,13 @@ struct Place {
 // elements g HD / 8 + j: each lane reads back only what it copied itself.  P
 // comes out as accumulators of S^T and is transposed 8 x 8 into B fragments.
 // A lane looks up the place of one group in 32 ahead of time.
+//
+// Bound, B200: one sequence of 131071 positions (32 heads on 8, size 128,
+// e4m3, bfloat16 rows) 66 us with its join, 4.1 TB/s, 63 % of the measured copy
+// rate: copies in flight and the ends of the one wave.  64 sequences of up to
+// 2048 (9 heads on 3, size 64, int8, float32) 17 us, 1.9 TB/s: 324 instructions
+// a group and the sequences' different lengths; two groups at once save
+// nothing.  300 positions of one sequence 6 us: latency.
 //
 // float32 rows (PIECES = 2) are the sum of two float16 pieces, which hold 22
 // bits of the row's largest element after a power of two has brought it to

@@ -22,6 +22,14 @@
 // which is rare after the first positions (bfloat16 rows do not even look for
 // a step's maximum otherwise).
 //
+// Three prompts of up to 1023 tokens behind 4000 positions (32 heads on 8, size
+// 128, int8, bfloat16 rows): 298 us, 637 TFLOP/s, 39 % of the measured bf16
+// rate; 360 tiles are 2.4 waves.  The chain of one tile, softmax and then its
+// two products, bounds a step (without the weights 222 us, without the
+// exponentials 289, without the conversion 316 of 332), then shared memory's
+// rate: 192 KB of operands, 64 KB of float16 stored and 64 KB of copies a step
+// of two tiles.
+//
 // Precision is that of the kernel for few rows (kv8.cu): float32 queries and
 // weights are two float16 pieces each, float16 queries one and their weights
 // two, bfloat16 ones one and one; the scales of K's and V's blocks enter the

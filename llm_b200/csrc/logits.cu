@@ -20,8 +20,10 @@
 // logit's word up and works out those that have one.  Bound by latency: a CTA
 // has about 10 K logits, so everything it reads first (logits, history,
 // biases, lengths) is asked for before the table is cleared, and there are
-// two barriers in all.  What is left of the time is instructions: 270 for 128
-// logits, a quarter of them divisions for single lanes.  The cluster's first CTA takes the largest of the CTAs'
+// two barriers in all.  64 rows of 151936 float32 logits with histories of up to
+// 4096: 38 us, 2.1 TB/s, 32 % of the measured copy rate (20 us without a
+// history): 270 instructions for 128 logits, of which counting and the
+// divisions of single lanes take 4 us each.  One row: 5.6 us, latency.  The cluster's first CTA takes the largest of the CTAs'
 // maxima; the others do not wait for it.
 #include <cooperative_groups.h>
 
