@@ -309,7 +309,11 @@ LLMB_API int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *ba
  * out_stride elements apart, 16-byte aligned; out must not overlap q unless
  * it is the same buffer with the same stride.  scale 0 means
  * 1 / sqrt(head_dim), negative ones are refused.  A row that sees no position becomes 0, one whose query
- * is not finite NaN; rows of no sequence stay as they were.  `workspace`:
+ * is not finite NaN; rows of no sequence stay as they were.  Positions whose
+ * block is not in the pool are not seen; a byte that is a NaN of e4m3 (append
+ * writes none) is no value of the cache.  (A wait inside the kernel that runs
+ * out after 1 s, which only a fault of the GPU can cause, makes the rows NaN.)
+ * `workspace`:
  * llmb_kv8_attention_workspace bytes of the caller's, 16-byte aligned, not
  * read before it is written; calls that may overlap on the GPU need their
  * own.  heads / kv_heads at most 64. */

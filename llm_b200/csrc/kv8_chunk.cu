@@ -661,9 +661,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                     }
                 }
             }
-            if (steps > 0) {  // nothing is in flight when tensor memory is given back
+            if (steps > 0) {  // nothing is in flight when tensor memory is given back, after a failure either
+                uint32_t never = 0;
                 commit(one, &bar.done);
-                bar_wait(&bar.done, 0, fail);
+                bar_wait(&bar.done, 0, &never);
             }
         } else if (warp == 13) {
             // Lane g has group g of 16 positions; a group without a block keeps what lies there, which is finite and gets no

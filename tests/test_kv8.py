@@ -623,6 +623,39 @@ def test_bounds_that_are_too_small_shift_nothing():
 
 
 @gpu
+def test_calls_at_once_on_two_streams():
+    """Decoding, a chunk and reads of two caches on two streams, each with its own workspace, as one after the other."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(15)
+    jobs = []
+    for lens, new, dtype in (([3000, 500], [1, 1], "f32"), ([900, 1500], [200, 300], "bf16")):
+        d = _filled(2, 64, 64, "int8", lens, rng)
+        q = _rows(torch, rng, sum(new), 14, 64, dtype)
+        batch, every = d.batch(lens, new, max_new=max(new)), d.batch(lens, lens)
+        out, k = torch.empty_like(q), torch.empty(sum(lens), 2, 64, device="cuda")
+        w = _workspace(d, batch, 14)
+
+        def job(d=d, q=q, batch=batch, every=every, out=out, k=k, w=w):
+            s = torch.cuda.current_stream().cuda_stream
+            d.cache.attention(batch, q, out, workspace=w, stream=s)
+            d.cache.read(every, k, stream=s)
+
+        job()
+        torch.cuda.synchronize()
+        jobs.append((job, out, out.clone(), k, k.clone()))
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        for (job, out, _, k, _), s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                out.fill_(7)
+                k.fill_(7)
+                job()
+        torch.cuda.synchronize()
+        for _, out, want, k, want_k in jobs:
+            assert torch.equal(out, want) and torch.equal(k, want_k)
+
+
+@gpu
 def test_refusals_on_the_device():
     """Host memory, a missing workspace, and no rows."""
     torch, _, _ = _t()
