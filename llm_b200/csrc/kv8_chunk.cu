@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bar.p[w]);
             }
-            if (ok && steps > 0) ok = bar_wait(&bar.o[w], 0, fail);
+            // (without a step, until the other warps' queries are where results go by)
+            if (ok) ok = bar_wait(steps > 0 ? &bar.o[w] : &bar.q[w], 0, fail);
             fence_after();
             ok = __all_sync(kFull, ok);
             // The rows' results, CW columns at a time by way of the tile's queries' place (their products are done), so that

@@ -465,6 +465,105 @@ def test_chunks(lens, new, dtype):
     _check_attention(d, lens, new, 4, dtype, stride=16)
 
 
+def _reference_by_head(d, lens, new, q, scale, window):
+    """_reference for many rows: a head's rows at once."""
+    torch, _, _ = _t()
+    grp = q.shape[1] // d.kv
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    size = torch.zeros(q.shape[0], 2, dtype=torch.float64, device="cuda")
+    at = 0
+    for i, (n, m) in enumerate(zip(lens, new)):
+        k, v = d.plain.rows(d.tables[i], n, n).double().cuda()
+        p, j = torch.arange(n - m, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+        seen = (j <= p) & (j > p - window) if window else j <= p
+        some = seen.any(1)
+        for h in range(q.shape[1] if n and m else 0):
+            qh, kh, vh = q[at:at + m, h].double().cuda(), k[:, h // grp], v[:, h // grp]
+            z = (scale * qh @ kh.T).masked_fill(~seen, -math.inf)
+            w = torch.where(some[:, None], torch.softmax(z, 1), 0.0)
+            out[at:at + m, h] = w @ vh
+            s = size[at:at + m]
+            s[:, 0] = s[:, 0].maximum((scale * qh.abs() @ kh.abs().T).masked_fill(~seen, 0).amax(1))
+            s[:, 1] = s[:, 1].maximum(vh.abs().amax())
+        at += m
+    return out.cpu(), size.cpu()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv,group,block,hd,cache", [(2, 4, 16, 64, "int8"), (1, 7, 128, 64, "e4m3"), (2, 3, 32, 128, "int8"),
+                                                     (1, 5, 64, 128, "e4m3")])
+def test_long_chunks(kv, group, block, hd, cache, dtype):
+    """Enough rows for the tensor cores' tiles: ragged, whole prompts and chunks behind a context, a sequence without
+    positions, one with more rows than positions, one of a single token; whole and in windows; one alone, in parts."""
+    torch, types, _ = _t()
+    rng = np.random.default_rng(kv * group + block)
+    heads = kv * group
+    for lens, new in (([1500, 0, 2, 900, 200], [400, 300, 1, 900, 260]), ([4000], [129])):
+        d = _filled(kv, block, hd, cache, lens, rng)
+        q = 1.5 * _rows(torch, rng, sum(new), heads, hd, dtype, 0.3)
+        for window in (0, 1, 333):
+            for bounds in (dict(), dict(max_new=max(new), max_len=max(lens))):
+                batch = d.batch(lens, new, **bounds)
+                out = torch.full_like(q, math.nan)
+                d.cache.attention(batch, q, out, window=window, workspace=_workspace(d, batch, heads))
+                want, size = _reference_by_head(d, lens, new, q.cpu(), 1 / math.sqrt(hd), window)
+                err, tol = (out.cpu().double() - want).abs(), _tolerance(size, max(lens), hd, dtype, want)
+                assert (err <= tol).all(), (lens, window, float(err.max()))
+                at = 0
+                for n, m in zip(lens, new):
+                    assert (out[at:at + max(m - n, 0)] == 0).all()  # rows before position 0
+                    at += m
+
+
+def _near(out, want, tol, dtype):
+    """Within the tolerance, or, where that reaches past the type's largest number, its infinity (float16 ends at 65504,
+    and rounding to nearest takes what is beyond to infinity)."""
+    torch, types, _ = _t()
+    got = out.cpu().double()
+    past = (want.abs() + tol >= torch.finfo(types[dtype]).max) & got.isinf() & (got.sign() == want.sign())
+    return ((got - want).abs() <= tol) | past
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_chunks_of_all_sizes(dtype):
+    """Scores that grow from step to step (the maximum has to follow), block scales that differ by 2^30, a query that is
+    not finite, and blocks without a place in the pool."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(16)
+    n, m, heads, hd = 2000, 300, 8, 64
+    d = Device(2, 32, hd, "int8", [n], rng)
+    k, v = (_rows(torch, rng, n, 2, hd, "f32", 0.3) for _ in range(2))
+    k *= torch.linspace(0, 12, n, device="cuda")[:, None, None]
+    v[320:640] *= 2.0 ** 30
+    v[1000:1032] = 0
+    d.append([n], [n], k, v)
+    q = _rows(torch, rng, m, heads, hd, dtype, 0.3)
+    q[7, 3, 5], q[250, 0, 0] = math.nan, math.inf
+    batch = d.batch([n], [m])
+    out = torch.empty_like(q)
+    d.cache.attention(batch, q, out, workspace=_workspace(d, batch, heads))
+    bad = torch.zeros(m, heads, dtype=torch.bool)
+    bad[7, 3] = bad[250, 0] = True
+    assert torch.isnan(out[bad.cuda()]).all()
+    want, size = _reference_by_head(d, [n], [m], q.cpu().nan_to_num(0, 0, 0), 1 / 8, 0)
+    assert _near(out, want, _tolerance(size, n, hd, dtype, want), dtype)[~bad].all()
+    # without its first blocks a sequence is the rest of it (window: none of the rows sees what is left out)
+    whole, cut = torch.empty_like(q), torch.empty_like(q)
+    d.cache.attention(batch, q, whole, window=700, workspace=_workspace(d, batch, heads))
+    tables = d.dtables.clone()
+    tables[0, :20] = torch.tensor([-1, len(d.k)] * 10, dtype=torch.int32)
+    gone = KV8Batch(torch.tensor([n], dtype=torch.int32).cuda(), tables, torch.tensor([0, m], dtype=torch.int32).cuda(), rows=m)
+    d.cache.attention(gone, q, cut, window=700, workspace=_workspace(d, gone, heads))
+    assert torch.equal(whole[~bad.cuda()], cut[~bad.cuda()])
+    d.cache.attention(gone, q, cut, workspace=_workspace(d, gone, heads))
+    d2 = Device(2, 32, hd, "int8", [n - 640], rng)
+    d2.append([n - 640], [n - 640], k[640:].contiguous(), v[640:].contiguous())
+    want, size = _reference_by_head(d2, [n - 640], [m], q.cpu().nan_to_num(0, 0, 0), 1 / 8, 0)
+    assert _near(cut, want, _tolerance(size, n, hd, dtype, want), dtype)[~bad].all()
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [1, 15, 16, 64, 700, 5000])
