@@ -230,16 +230,36 @@ void append_launch(const Kv8 &c, const void *k, const void *v, int64_t row_strid
     else k_kv8_append<T, E4M3, HD, HD * (int)sizeof(T) / 32><<<grid, 256, 0, st>>>(c, kp, vp, row_stride, tiles);
 }
 
+// The four 8-bit values of w as two pairs of float16, exactly (bytes 0 and 1, bytes 2 and 3).
+template <bool E4M3>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (E4M3) {
+        asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    } else {  // u = q + 128 under 1024's exponent is 1024 + u
+        const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 k = __half2half2(__float2half_rn(1152.f));
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), k), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), k);
+        lo = *reinterpret_cast<const uint32_t *>(&x), hi = *reinterpret_cast<const uint32_t *>(&y);
+    }
+}
+
 // --------------------------------------------------------------- read --
 
 // One block of a sequence and `tiles` of its 2 kv_heads tiles, 16 bytes of
-// result a thread and step, four steps' loads in flight.  Bound by the
-// memory's rate: 352 MB, two thirds of them written, in 74 us, 73 % of the
-// measured copy rate (eight steps in flight: the same).
+// result a thread and step, two steps' loads in flight.  A thread keeps its
+// place in a row: its steps are whole rows and whole tiles apart, so that
+// addresses cost additions only.  Bound by the memory's rate: 352 MB of 32 x
+// 128 tiles of e4m3, two thirds of them written, in 66 us, 82 % of the measured
+// copy rate, and 202 MB of 64 x 128 tiles of int8 in 46 us (with a division a
+// step and 48 registers 76 and 49 us; four steps in flight: 70 and 46).  The
+// conversions are the ones that measured best here: of e4m3 the machine's own
+// (by shifts and a factor 72 us), of int8 by kv8_half2 (by `halves` 54 us).
 template <class T, bool E4M3, int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k, T *__restrict__ v,
                                                   int64_t row_stride, int tiles) {
-    constexpr int E = 16 / (int)sizeof(T), PR = HD / E, N = 4;  // values of a step, steps of a row, steps in flight
+    constexpr int E = 16 / (int)sizeof(T), PR = HD / E, N = 2;  // values of a step, steps of a row, steps in flight
     const int s = blockIdx.z;
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
@@ -248,35 +268,53 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
     if (p0 >= end) return;
     const int b = kv8_block(c, s, j);
     const int lo = max(q.first - p0, 0), hi = min(end - p0, c.block);
-    const int64_t row = (int64_t)(q.start + p0 - q.first) * row_stride;
-    const int t0 = blockIdx.y * tiles, t1 = min(t0 + tiles, 2 * c.kvh), per = c.block * PR;
-    const int shift = c.bshift + (PR == 32 ? 5 : PR == 16 ? 4 : 3);  // of `per`, a power of two
-    for (int u0 = threadIdx.x; u0 < (t1 - t0) * per; u0 += N * blockDim.x) {
+    // the threads take 256 / per tiles at once, or a tile in per / 256 steps (both powers of two)
+    const int shift = c.bshift + (PR == 32 ? 5 : PR == 16 ? 4 : 3), per = 1 << shift;
+    const int steps = shift > 8 ? shift - 8 : 0, at_once = shift < 8 ? 8 - shift : 0;  // (their logarithms)
+    const int in_tile = threadIdx.x & (per - 1), row0 = in_tile / PR, rows = min(per, 256) / PR;
+    const int t0 = blockIdx.y * tiles + ((int)threadIdx.x >> min(shift, 8)), t1 = min((int)(blockIdx.y + 1) * tiles, 2 * c.kvh);
+    const int64_t to = (int64_t)(q.start + p0 - q.first + row0) * row_stride + in_tile % PR * E;
+    const int64_t from = (b < 0 ? 0 : b * c.bstride) + in_tile * E, apart = (int64_t)rows * row_stride;
+    const float *ks = c.ks + (b < 0 ? 0 : (int64_t)b * c.kvh), *vs = c.vs + (b < 0 ? 0 : (int64_t)b * c.kvh);
+    const int n = t1 > t0 ? (((t1 - t0 - 1) >> at_once) + 1) << steps : 0;
+    for (int i0 = 0; i0 < n; i0 += N) {
         uint2 w[N];
         float sc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = u0 + i * blockDim.x, t = t0 + (u >> shift), e = u & (per - 1);
+            const int t = t0 + ((i0 + i) >> steps << at_once), y = (i0 + i) & ((1 << steps) - 1);
             w[i] = make_uint2(0, 0), sc[i] = 0.f;
-            if (t < t1 && b >= 0) {
-                const uint8_t *src = (t & 1 ? c.v : c.k) + b * c.bstride + (int64_t)(t >> 1) * c.block * HD + e * E;
+            if (i0 + i < n && b >= 0) {
+                const uint8_t *src = (t & 1 ? c.v : c.k) + from + ((t >> 1) * c.block + y * rows) * HD;
                 if constexpr (E == 8) w[i] = __ldg(reinterpret_cast<const uint2 *>(src));
                 else w[i].x = __ldg(reinterpret_cast<const uint32_t *>(src));
-                sc[i] = __ldg((t & 1 ? c.vs : c.ks) + (int64_t)b * c.kvh + (t >> 1));
+                sc[i] = __ldg((t & 1 ? vs : ks) + (t >> 1));
             }
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = u0 + i * blockDim.x, t = t0 + (u >> shift), e = u & (per - 1), r = e / PR;
+            const int t = t0 + ((i0 + i) >> steps << at_once), y = (i0 + i) & ((1 << steps) - 1), r = row0 + y * rows;
             T *dst = t & 1 ? v : k;
-            if (t >= t1 || r < lo || r >= hi || !dst) continue;
-            float f[4], h[4];
-            kv8_floats<E4M3>(w[i].x, f);
-            if (E == 8) kv8_floats<E4M3>(w[i].y, h);
+            if (i0 + i >= n || r < lo || r >= hi || !dst) continue;
+            const uint32_t words[2] = {w[i].x, w[i].y};
             T o[E];
 #pragma unroll
-            for (int z = 0; z < E; ++z) o[z] = kv8_from<T>(b < 0 ? 0.f : __fmul_rn(z < 4 ? f[z & 3] : h[z & 3], sc[i]));
-            *reinterpret_cast<uint4 *>(dst + row + (int64_t)r * row_stride + (t >> 1) * HD + e % PR * E) = *reinterpret_cast<const uint4 *>(o);
+            for (int z = 0; z < E; z += 4) {
+                float f[4];
+                if constexpr (E4M3) {
+                    uint32_t h[2];
+                    halves<true>(words[z / 4], h[0], h[1]);
+                    const float2 x0 = __half22float2(*reinterpret_cast<const __half2 *>(&h[0]));
+                    const float2 x1 = __half22float2(*reinterpret_cast<const __half2 *>(&h[1]));
+                    f[0] = x0.x, f[1] = x0.y, f[2] = x1.x, f[3] = x1.y;
+                } else {
+                    kv8_floats<false>(words[z / 4], f);
+                }
+                // (no block: a byte 0 is the value 0, and the scale is 0)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[z + x] = kv8_from<T>(__fmul_rn(f[x], sc[i]));
+            }
+            *reinterpret_cast<uint4 *>(dst + to + y * apart + (t >> 1) * HD) = *reinterpret_cast<const uint4 *>(o);
         }
     }
 }
@@ -301,21 +339,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// The four 8-bit values of w as two pairs of float16, exactly (bytes 0 and 1, bytes 2 and 3).
-template <bool E4M3>
-__device__ __forceinline__ void halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if (E4M3) {
-        asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    } else {  // u = q + 128 under 1024's exponent is 1024 + u
-        const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 k = __half2half2(__float2half_rn(1152.f));
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), k), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), k);
-        lo = *reinterpret_cast<const uint32_t *>(&x), hi = *reinterpret_cast<const uint32_t *>(&y);
-    }
 }
 
 // What 16 positions share: where they lie in the pools (below 0: nowhere), K's scale, V's scale = mv 2^lv with 2^-lv.
