@@ -427,11 +427,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 4 : 2) k_kv8_attend(
         x.at = b * c.bstride + ((int64_t)head * c.block + (p & (c.block - 1))) * HD;
         x.ks = __ldg(c.ks + (int64_t)b * c.kvh + head);
         const float vs = __ldg(c.vs + (int64_t)b * c.kvh + head);
-        const bool normal = vs >= FLT_MIN && vs <= FLT_MAX;  // (smaller ones, 0 among them, are factors as they are)
-        const uint32_t u = __float_as_uint(vs);
-        const int ex = normal ? (int)(u >> 23) - 127 : 0;
-        x.lv = (float)ex, x.mv = normal ? __uint_as_float((u & 0x7fffffu) | 0x3f800000u) : vs;
-        x.unlv = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
+        const int ex = kv8_v_scale(vs, x.mv);
+        x.lv = (float)ex, x.unlv = kv8_pow2(-ex);
         return x;
     };
     auto of_lane = [&](const Place &x, int i) {

@@ -116,6 +116,17 @@ __device__ __forceinline__ bool kv8_query_scale(uint32_t m, float &up, float &do
     return fine;
 }
 
+// V's scale as mv 2^ex: mv is in [1, 2) for every scale that append makes (2^-109 to 2^121, and 0 with mv 0), smaller for
+// smaller ones, and has the scale's sign; ex is at least kKv8LeastExp.
+constexpr int kKv8LeastExp = -109;
+__device__ __forceinline__ float kv8_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ int kv8_v_scale(float vs, float &mv) {
+    const uint32_t u = __float_as_uint(vs) & 0x7fffffffu;
+    const int ex = u == 0 || u >= 0x7f800000u ? 0 : min(max((int)(u >> 23) - 127, kKv8LeastExp), 126);
+    mv = vs * kv8_pow2(-ex);
+    return ex;
+}
+
 constexpr int kKv8MaxGroup = 64;  // query heads of one kv head
 
 // ---- the attention's split of positions, as both its kernels see it

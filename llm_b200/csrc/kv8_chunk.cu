@@ -62,7 +62,9 @@ template <> constexpr int kQPieces<float> = 2;
 template <class T> constexpr int kPPieces = 2;
 template <> constexpr int kPPieces<__nv_bfloat16> = 1;
 
-// What 16 positions share: K's scale; V's scale = mv 2^lv, with 2^-lv.
+// What 16 positions share: K's scale; V's scale = mv 2^lv, with 2^-lv.  bfloat16 rows, whose precision leaves room for the
+// rounding of a logarithm, have all of the scale in lv, and mv is not used; a scale that has no logarithm, or is below all
+// that append makes, makes the group's values 0 for them as they are stored for the products.
 struct Group {
     float ks, lv, mv, unlv;
 };
@@ -91,7 +93,7 @@ struct Layout {
 
 struct Bars {
     uint64_t full[4], empty[4], raw[8], free[8], group[8], s[2], p[2], q[2], o[2], done;
-    uint32_t tmem, fail;
+    uint32_t tmem, fail, none[8];  // none: a step's groups whose values are 0, a bit each
 };
 static_assert(sizeof(Bars) <= 384, "the barriers' space");
 
@@ -588,6 +590,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
             uint4 x[NP];
 #pragma unroll
             for (int n = 0; n < NP; ++n) x[n] = *reinterpret_cast<const uint4 *>(src + n * 2048);
+            if (PP == 1 && (i & 1)) {
+                if (const uint32_t none = bar.none[(i >> 1) & 7])  // (written before the wait for these copies began)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+                        if (none >> ((key0 + n * (128 / PC)) >> 4) & 1) x[n] = make_uint4(0, 0, 0, 0);
+            }
             __syncwarp();
             if (lane == 0) bar_arrive(&bar.free[i % D]);
 #pragma unroll
@@ -689,6 +697,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 for (int i = 2 * j; i < 2 * j + 2; ++i) {
                     ok = i < D || bar_wait(&bar.free[i % D], (i / D - 1) & 1, fail);
                     if (!(ok = __all_sync(kFull, ok))) break;
+                    if (PP == 1 && (i & 1)) {
+                        const uint32_t none = __ballot_sync(kFull, b >= 0 && !(vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX));
+                        if (lane == 0) bar.none[j & 7] = none;
+                    }
                     if (lane == 0) bar_expect(&bar.raw[i % D], bytes);
                     __syncwarp();
                     if (first) bulk(smem + L::raw + (i % D) * 128 * HD + lane * 16 * HD, (i & 1 ? c.v : c.k) + off, n * 16 * HD, &bar.raw[i % D]);
@@ -698,17 +710,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 // The groups' scales.  Their place was last read in step j - 8, which was over: this step's V is copied to
                 // where V of step j - copies / 2 was, after that was stored to a slot, after the products that used the
                 // slot before, of a step j - 6 at the earliest, and so the weights of the step before that, were done.
+                // (So was the converters' look at none: they had V of step j - copies / 2 by then.)
                 if (lane < 8) {
                     Group g = {0.f, -INFINITY, 0.f, 0.f};  // no block: -inf as a score
                     if (b >= 0) {
-                        const bool has = vs > 0.f;
-                        g.ks = ks;
-                        if (PP == 2) {
-                            const int lv = has ? ilogbf(vs) : 0;
-                            g.lv = (float)lv, g.mv = has ? scalbnf(vs, -lv) : vs, g.unlv = scalbnf(1.f, -lv);
-                        } else {  // bfloat16's precision leaves room for the rounding of a logarithm
-                            g.lv = has ? log2f(vs) : 0.f, g.mv = 1.f, g.unlv = has ? 1.f / vs : 1.f;
-                        }
+                        const int ex = kv8_v_scale(vs, g.mv);
+                        g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex);
+                        if (PP == 1 && vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = 1.f / vs;
                     }
                     groups[(j & 7) * 8 + lane] = g;
                 }

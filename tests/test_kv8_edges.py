@@ -1,0 +1,59 @@
+"""The 8-bit key/value cache where callers' own scales, windows and bounds reach its limits.
+
+Helpers, the plain restatement and the tolerances are test_kv8.py's.
+"""
+
+import math
+
+import numpy as np
+import pytest
+
+from tests.test_kv8 import DTYPES, _filled, _reference_by_head, _rows, _t, _tolerance, _workspace
+
+gpu = pytest.mark.gpu
+
+
+def _scale(d, kind, table, values):
+    """Gives the blocks of a sequence other scales over the bytes they have: values for its first blocks."""
+    torch, _, _ = _t()
+    for b, s in zip(table, values):
+        (d.ks, d.vs)[kind][b] = s
+        d.plain.scale[kind, b] = s
+
+
+def _attention(d, lens, new, heads, dtype, q, window=0):
+    """(result, float64 reference, tolerance)"""
+    torch, _, _ = _t()
+    batch = d.batch(lens, new)
+    out = torch.full_like(q, math.nan)
+    d.cache.attention(batch, q, out, window=window, workspace=_workspace(d, batch, heads))
+    want, size = _reference_by_head(d, lens, new, q.cpu(), 1 / math.sqrt(d.hd), window)
+    return out.cpu().double(), want, _tolerance(size, max(lens), d.hd, dtype, want)
+
+
+# Rows of the call: one token (the kernel for few rows) and enough for the tensor cores' tiles.
+ROWS = (1, 400)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("cache,hd", [("int8", 64), ("e4m3", 128)])
+def test_a_scale_of_0_makes_values_0_whatever_the_bytes(cache, hd, rows, dtype):
+    """Blocks whose V scale a caller cleared, or made smaller than float32's normal numbers, are as read gives them in
+    the attention too, and their positions count in the softmax."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(21)
+    n, kv, heads = 1500, 2, 8
+    d = _filled(kv, 32, hd, cache, [n], rng)
+    _scale(d, 1, d.tables[0][3::5], [0.0, 2.0 ** -130, 0.0, 2.0 ** -149, 2.0 ** -115, 0.0])
+    k, v = (torch.empty(n, kv, hd, device="cuda") for _ in range(2))
+    d.cache.read(d.batch([n], [n]), k, v)
+    assert torch.equal(v.cpu(), d.plain.rows(d.tables[0], n, n)[1]) and (v[96:128] == 0).all()
+    q = _rows(torch, rng, rows, heads, hd, dtype, 0.3)
+    got, want, tol = _attention(d, [n], [rows], heads, dtype, q)
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+    # and where no block has a scale, the result is 0
+    _scale(d, 1, d.tables[0], [0.0] * len(d.tables[0]))
+    got, _, _ = _attention(d, [n], [rows], heads, dtype, q)
+    assert (got == 0).all()
