@@ -420,14 +420,17 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 4 : 2) k_kv8_attend(
     const int all0 = a.window > 0 ? max(sq.first + tok1 + 1 - a.window, lo) : lo, all1 = min(sq.first + tok0 + 1, hi);
 
     constexpr int step = 16 * kAttWarps;
-    auto look_up = [&](int p) {
+    int low = kKv8NoExp;
+    auto look_up = [&](int p) {  // by the whole warp
         Place x = {-1, 0.f, 0.f, 0.f, 0.f};
         const int b = p < hi ? kv8_block(c, s, p >> c.bshift) : -1;
-        if (b < 0) return x;
-        x.at = b * c.bstride + ((int64_t)head * c.block + (p & (c.block - 1))) * HD;
-        x.ks = __ldg(c.ks + (int64_t)b * c.kvh + head);
-        const float vs = __ldg(c.vs + (int64_t)b * c.kvh + head);
-        const int ex = kv8_v_scale(vs, x.mv);
+        float vs = 0.f;
+        if (b >= 0) {
+            x.at = b * c.bstride + ((int64_t)head * c.block + (p & (c.block - 1))) * HD;
+            x.ks = __ldg(c.ks + (int64_t)b * c.kvh + head);
+            vs = __ldg(c.vs + (int64_t)b * c.kvh + head);
+        }
+        const int ex = kv8_v_scale(vs, x.mv, low);
         x.lv = (float)ex, x.unlv = kv8_pow2(-ex);
         return x;
     };

@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 const int p = lo + j * kKeys + 16 * lane;
                 return lane < 8 && p < hi ? kv8_block(c, s, p >> c.bshift) : -1;
             };
-            int b = steps > 0 ? block_of(0) : -1, sent = 0;
+            int b = steps > 0 ? block_of(0) : -1, sent = 0, low = kKv8NoExp;
             for (int j = 0; ok && j < steps; ++j) {
                 const int ahead = j + 1 < steps ? block_of(j + 1) : -1;
                 const int64_t off = b < 0 ? 0 : b * c.bstride + ((int64_t)head * c.block + ((lo + j * kKeys + 16 * lane) & (c.block - 1))) * HD;
@@ -711,15 +711,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 // where V of step j - copies / 2 was, after that was stored to a slot, after the products that used the
                 // slot before, of a step j - 6 at the earliest, and so the weights of the step before that, were done.
                 // (So was the converters' look at none: they had V of step j - copies / 2 by then.)
-                if (lane < 8) {
-                    Group g = {0.f, -INFINITY, 0.f, 0.f};  // no block: -inf as a score
-                    if (b >= 0) {
-                        const int ex = kv8_v_scale(vs, g.mv);
-                        g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex);
-                        if (PP == 1 && vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = 1.f / vs;
-                    }
-                    groups[(j & 7) * 8 + lane] = g;
+                Group g = {0.f, -INFINITY, 0.f, 0.f};  // no block: -inf as a score
+                const int ex = kv8_v_scale(vs, g.mv, low);
+                if (b >= 0) {
+                    g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex);
+                    if (PP == 1 && vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = 1.f / vs;
                 }
+                if (lane < 8) groups[(j & 7) * 8 + lane] = g;
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bar.group[j & 7]);
                 b = ahead;

@@ -8,7 +8,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_kv8 import DTYPES, _filled, _reference_by_head, _rows, _t, _tolerance, _workspace
+from tests.test_kv8 import DTYPES, Device, _filled, _reference_by_head, _rows, _t, _tolerance, _workspace
 
 gpu = pytest.mark.gpu
 
@@ -57,3 +57,28 @@ def test_a_scale_of_0_makes_values_0_whatever_the_bytes(cache, hd, rows, dtype):
     _scale(d, 1, d.tables[0], [0.0] * len(d.tables[0]))
     got, _, _ = _attention(d, [n], [rows], heads, dtype, q)
     assert (got == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,size", [("f32", 2.0 ** -40), ("f32", 2.0 ** 20), ("f16", 2.0 ** -9), ("bf16", 2.0 ** -40),
+                                        ("bf16", 2.0 ** 30)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("zeros", ["between", "before"])
+def test_blocks_of_zeros_beside_values_of_any_size(zeros, rows, dtype, size):
+    """Positions whose values are all 0 take their part of the softmax and nothing of the others' precision: between
+    blocks of small or large values, and where a part of the positions starts with thousands of them."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(22)
+    n, kv, heads, hd = 6000, 1, 4, 64
+    d = Device(kv, 16, hd, "int8", [n], rng)
+    k, v = (_rows(torch, rng, n, kv, hd, "f32", 0.3) for _ in range(2))
+    v *= size
+    if zeros == "between":
+        for at in (0, 320, 1024, 4000):
+            v[at:at + 32] = 0
+    else:
+        v[:4096] = 0
+    d.append([n], [n], k, v)
+    q = _rows(torch, rng, rows, heads, hd, dtype, 0.3)
+    got, want, tol = _attention(d, [n], [rows], heads, dtype, q)
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
