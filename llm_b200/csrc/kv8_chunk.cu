@@ -62,9 +62,9 @@ template <> constexpr int kQPieces<float> = 2;
 template <class T> constexpr int kPPieces = 2;
 template <> constexpr int kPPieces<__nv_bfloat16> = 1;
 
-// What 16 positions share: K's scale; V's scale = mv 2^lv, with 2^-lv.  bfloat16 rows, whose precision leaves room for the
-// rounding of a logarithm, have all of the scale in lv, and mv is not used; a scale that has no logarithm, or is below all
-// that append makes, makes the group's values 0 for them as they are stored for the products.
+// What 16 positions share: K's scale; V's scale = mv 2^lv, with 2^-lv in the unit of the weights' sums.  bfloat16 rows, whose
+// precision leaves room for the rounding of a logarithm, have all of the scale in lv, and mv is not used; a scale that has
+// no logarithm, or is below all that append makes, makes the group's values 0 for them as they are stored for the products.
 struct Group {
     float ks, lv, mv, unlv;
 };
@@ -386,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
     constexpr int PN = HD / 64, QP = kQPieces<T>, PP = kPPieces<T>, NS = L::slots, SUM = kSumSteps<T>;
     constexpr int ROWS = 128 * L::tiles, SUM1 = SUM > 0 ? SUM : 1;
     constexpr float unit = E4M3 ? 256.f : 1.f;
+    constexpr float SU = PP == 1 ? 1.f / 256.f : 1.f;  // the unit of the weights' sums: 1 / vs is up to 2^109, 2^-ex up to 2^101
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars &bar = *reinterpret_cast<Bars *>(smem + L::bars);
     Group *groups = reinterpret_cast<Group *>(smem + L::group);
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
             const bool split = a.splits > 1;
             // where the lane's row goes (-1: nowhere), and the rows that it stores pieces of
             const int64_t own = !on ? -1 : split ? part * HD : (int64_t)(sq.start + tok) * a.out_stride + h * HD;
-            const float inv = split ? unit : l == 0.f ? 0.f : unit / l;
+            const float inv = split ? unit * SU : l == 0.f ? 0.f : unit * SU / l;
             if (on && split) a.part_ml[part] = make_float2(m, ok ? l : NAN);
 #pragma unroll 1
             for (int k = 0; k < HD / CW; ++k) {
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                     ok = i < D || bar_wait(&bar.free[i % D], (i / D - 1) & 1, fail);
                     if (!(ok = __all_sync(kFull, ok))) break;
                     if (PP == 1 && (i & 1)) {
-                        const uint32_t none = __ballot_sync(kFull, b >= 0 && !(vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX));
+                        const uint32_t none = __ballot_sync(kFull, b >= 0 && !(vs >= kv8_pow2(kKv8LeastScale) && vs <= FLT_MAX));
                         if (lane == 0) bar.none[j & 7] = none;
                     }
                     if (lane == 0) bar_expect(&bar.raw[i % D], bytes);
@@ -714,8 +715,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 Group g = {0.f, -INFINITY, 0.f, 0.f};  // no block: -inf as a score
                 const int ex = kv8_v_scale(vs, g.mv, low);
                 if (b >= 0) {
-                    g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex);
-                    if (PP == 1 && vs >= kv8_pow2(kKv8LeastExp) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = 1.f / vs;
+                    g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex) * SU;
+                    if (PP == 1 && vs >= kv8_pow2(kKv8LeastScale) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = SU / vs;
                 }
                 if (lane < 8) groups[(j & 7) * 8 + lane] = g;
                 __syncwarp();

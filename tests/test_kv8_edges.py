@@ -82,3 +82,22 @@ def test_blocks_of_zeros_beside_values_of_any_size(zeros, rows, dtype, size):
     q = _rows(torch, rng, rows, heads, hd, dtype, 0.3)
     got, want, tol = _attention(d, [n], [rows], heads, dtype, q)
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", ROWS)
+def test_many_of_the_smallest_values(rows, dtype):
+    """20000 positions of values just above 2^-100, the least that append keeps: the sum of the weights, in which the
+    scale's inverse stands, stays finite."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(23)
+    n, kv, heads, hd = 20000, 1, 2, 64
+    d = Device(kv, 128, hd, "e4m3", [n], rng)
+    k = 0.01 * _rows(torch, rng, n, kv, hd, "f32", 0.0)
+    v = 2.0 ** -100 * (1 + 0.01 * torch.rand(n, kv, hd, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    d.append([n], [n], k, v)
+    assert float(d.vs[torch.from_numpy(d.tables[0]).long()].min()) >= 2.0 ** -109
+    q = _rows(torch, rng, rows, heads, hd, dtype, 0.0)
+    got, want, tol = _attention(d, [n], [rows], heads, dtype, q)
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
