@@ -279,15 +279,18 @@ typedef struct {
 /* Writes the rows of k and v (n_rows rows of [kv_heads][head_dim] elements
  * of `type`, row_stride elements apart, 16-byte aligned) into the cache.  Per
  * block and head, with M = 127 (int8) or 448 (e4m3): a block's first rows
- * give it the scale a * (1 / M), a their largest magnitude.  Rows that come later
- * and do not fit (a > M scale) grow the scale by the smallest power of two
- * that fits, and the values already there are rounded to the new step: all
- * the roundings of a value together stay within one step, however the rows
- * came.  (A scale that would grow more than 2^20-fold starts anew at a * (1 / M);
- * the earlier values are 0 then.)  Values round to nearest even.  An infinity
- * is stored as M steps and a NaN as 0, neither counts for a; a below 2^-100
- * is stored as 0.  A sequence's blocks that receive rows must belong to it
- * alone; blocks outside the table's range or the pool are skipped. */
+ * give it the scale a * (1 / M), a their largest magnitude.  Rows that come
+ * later and do not fit grow the scale by the smallest power of two that fits,
+ * and the values already there are rounded to the new step: all the roundings
+ * of a value together stay within one step, however the rows came.  (a fits
+ * where a <= (M + 2^-12) scale, so that it fits the scale made for it, however
+ * that was rounded.  A scale that would grow more than 2^20-fold starts anew
+ * at a * (1 / M); the earlier values are 0 then.)  Values round to nearest
+ * even.  An infinity is stored as M steps and a NaN as 0, neither counts for
+ * a.  Where a is below 2^-100 the scale stays as it is: rows of a block
+ * without one are stored as 0, others are rounded to its step (and saturate at
+ * M steps).  A sequence's blocks that receive rows must belong to it alone;
+ * blocks outside the table's range or the pool are skipped. */
 LLMB_API int llmb_kv8_append(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *k, const void *v,
                              int type, int64_t row_stride, void *stream);
 

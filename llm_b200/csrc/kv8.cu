@@ -27,8 +27,8 @@ constexpr float kFit = 1.f / 4096.f;        // a scale still fits top + kFit ste
 constexpr float kTiny = 7.888609052e-31f;   // 2^-100
 constexpr float kRestart = 1048576.f;       // 2^20
 
-// Four values to 8 bits: to the nearest, ties to even, saturated; NaN becomes 0.  FINITE: none of them is infinite or NaN
-// and none above the top by more than the scale's rounding, so that rounding alone ends at the top.
+// Four values to 8 bits: to the nearest, ties to even, saturated; NaN becomes 0.  FINITE: none of the products is infinite or
+// NaN and none above the top by more than a quarter, so that rounding alone ends at the top.
 template <bool E4M3, bool FINITE>
 __device__ __forceinline__ uint32_t kv8_pack(const float (&x)[4], float inv) {
     float y[4];
@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8 c, const T *__rest
                 }
             }
         };
-        finite ? write(std::true_type{}) : write(std::false_type{});
+        // (rows below kTiny take a scale as it is, and one of the caller's may be too small for them, its inverse infinite)
+        finite && __fmul_rn(a, inv) <= kv8_top<E4M3>() + 0.25f ? write(std::true_type{}) : write(std::false_type{});
         if (old != 1.f)
             for (int u = threadIdx.x; u < lo * HD / 4; u += blockDim.x) {
                 uint32_t *w = reinterpret_cast<uint32_t *>(tile) + u;

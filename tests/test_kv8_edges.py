@@ -101,3 +101,31 @@ def test_many_of_the_smallest_values(rows, dtype):
     q = _rows(torch, rng, rows, heads, hd, dtype, 0.0)
     got, want, tol = _attention(d, [n], [rows], heads, dtype, q)
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cache", ["int8", "e4m3"])
+def test_append_behind_scales_of_the_callers(cache, dtype):
+    """Rows below 2^-100 leave a block's scale as it is; where that is smaller than they need they saturate, and no byte
+    is a NaN or has another sign, down to scales whose inverse is not finite."""
+    torch, types, caches = _t()
+    rng = np.random.default_rng(24)
+    kv, block, hd = 2, 16, 64
+    scales = [2.0 ** -107, 2.0 ** -112, 2.0 ** -126, 2.0 ** -130, 2.0 ** -149, 2.0 ** -90, 1.0]
+    for size in (0.0, 2.0 ** -101, 2.0 ** -105, 2.0 ** -125):
+        d = Device(kv, block, hd, cache, [9] * len(scales), rng)
+        n = len(scales)
+        d.append([5] * n, [5] * n, *(_rows(torch, rng, 5 * n, kv, hd, "f32") for _ in range(2)))
+        for i, s in enumerate(scales):
+            for kind in range(2):
+                _scale(d, kind, d.tables[i], [s])
+        x = torch.from_numpy(rng.uniform(0.3, 0.9, (4 * n, kv, hd)).astype(np.float32))
+        x[1::3] *= -1
+        x = (x * size).to(types[dtype]).cuda()
+        with np.errstate(over="ignore"):  # (the restatement's inverse)
+            d.append([9] * n, [4] * n, x, -x)
+        d.same_as_plain([9] * n)
+        bytes_ = d.k.view(torch.uint8)[torch.from_numpy(d.tables[:, 0]).long(), :, :9]
+        if cache == "e4m3":
+            assert not ((bytes_ & 0x7f) == 0x7f).any()
