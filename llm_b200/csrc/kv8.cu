@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 4 : 2) k_kv8_attend(
     lo += blockIdx.x * a.part;
     hi = min(hi, lo + a.part);
     // every row sees all of [all0, all1)
-    const int all0 = a.window > 0 ? max(sq.first + tok1 + 1 - a.window, lo) : lo, all1 = min(sq.first + tok0 + 1, hi);
+    const int all0 = max(kv8_first_seen(sq.first + tok1, a.window), lo), all1 = min(sq.first + tok0 + 1, hi);
 
     constexpr int step = 16 * kAttWarps;
     int low = kKv8NoExp;
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 4 : 2) k_kv8_attend(
         for (int e = 0; e < 2; ++e) {
             fac[i][e] = __shfl_sync(kFull, f, 4 * (2 * t + e));
             const int r2 = row0 + 8 * i + 2 * t + e;
-            pos[i][e] = r2 <= last ? sq.first + r2 / a.group : -1;
+            pos[i][e] = r2 <= last ? max(sq.first + r2 / a.group, -1) : -1;  // (less any window it is an int)
         }
     }
 

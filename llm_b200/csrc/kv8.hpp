@@ -154,10 +154,13 @@ struct Kv8Att {
     float *part_o;    // [rows][heads][splits][head_dim]
 };
 
+// The first position that a row at position pos sees (pos may be below 0, and the window the largest integer).
+__device__ __forceinline__ int kv8_first_seen(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 // Positions [lo, hi) that the tokens t0 .. t1 (inclusive) of a sequence see between them; lo a multiple of 16.
 __device__ __forceinline__ void kv8_span(const Kv8Seq &q, int window, int t0, int t1, int &lo, int &hi) {
     hi = max(min(q.first + t1 + 1, q.len), 0);
-    lo = window > 0 ? max(q.first + t0 + 1 - window, 0) & ~15 : 0;
+    lo = kv8_first_seen(q.first + t0, window) & ~15;
     if (lo > hi) lo = hi;
 }
 

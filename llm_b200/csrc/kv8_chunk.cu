@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
             for (int j = 0; j < steps; ++j) {
                 const int p0 = lo + j * kKeys;
                 // the row sees positions p0 + [b0, b1)
-                const int b1 = min(min(pos + 1, hi) - p0, kKeys), b0 = a.window > 0 ? max(pos + 1 - a.window - p0, 0) : 0;
+                const int b1 = min(min(pos + 1, hi) - p0, kKeys), b0 = max(kv8_first_seen(pos, a.window) - p0, 0);
                 const bool whole = __all_sync(kFull, b0 == 0 && b1 == kKeys);
                 ok = bar_wait(&bar.group[j & 7], (j >> 3) & 1, fail) && bar_wait(&bar.s[w], j & 1, fail);
                 if (!(ok = __all_sync(kFull, ok))) break;

@@ -129,3 +129,21 @@ def test_append_behind_scales_of_the_callers(cache, dtype):
         bytes_ = d.k.view(torch.uint8)[torch.from_numpy(d.tables[:, 0]).long(), :, :9]
         if cache == "e4m3":
             assert not ((bytes_ & 0x7f) == 0x7f).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,new,heads", [([10, 700], [14, 3], 2), ([900, 40], [1000, 300], 8)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 16385, 5])
+def test_windows_up_to_the_largest_integer(window, lens, new, heads, dtype):
+    """The largest window is none, also for sequences with more rows than positions, whose first rows see nothing."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(25)
+    d = _filled(2, 16, 64, "int8", lens, rng)
+    q = _rows(torch, rng, sum(new), heads, 64, dtype, 0.3)
+    got, want, tol = _attention(d, lens, new, heads, dtype, q, window=window)
+    assert ((got - want).abs() <= tol).all()
+    if window > 5:
+        whole, _, _ = _attention(d, lens, new, heads, dtype, q)
+        # (another window may cut the positions into other parts: two results within their tolerance)
+        assert ((got - whole).abs() <= 2 * tol).all() and (got[:new[0] - lens[0]] == 0).all()
