@@ -937,13 +937,23 @@ struct Cut {
 // Parts of the kernel for many rows: one CTA takes an SM, so with `units` CTAs of one part each the last wave may be
 // nearly empty; parts fill it, at the price of the join.  Measured on a B200: a step of 128 positions 3 us, a CTA's start
 // 4 us, the join 3 us and its traffic at 4 TB/s.
+double join_us(int64_t slots, int hd) { return (double)slots * hd * 8 / 4e6; }  // for each part
+
+// No more parts than these can be the least time.  s parts take units s / 148 waves or more, of steps / s steps or more, one
+// takes less than units / 148 + 1: s parts gain less than 3 steps + 4 - 4 (s - 1) units / 148, and their join costs 3 + s join_us.
+int chunk_most_parts(int64_t units, int64_t span, int64_t slots, int hd) {
+    const double steps = (double)((span + 127) / 128), wave = 4.0 * (double)units / 148;
+    return (int)std::max(std::min({(3 * steps + 1 + wave) / (wave + join_us(slots, hd)), steps, 64.0}), 1.0);
+}
+
 int chunk_parts(int64_t units, int64_t span, int64_t slots, int hd) {
     const int64_t steps = (span + 127) / 128;
+    const int most = chunk_most_parts(units, span, slots, hd);
     int best = 1;
     double least = 0;
-    for (int s = 1; s <= 64 && s <= steps; ++s) {
+    for (int s = 1; s <= most; ++s) {
         const double waves = (double)((units * s + 147) / 148);
-        const double us = waves * (3.0 * (double)((steps + s - 1) / s) + 4.0) + (s > 1 ? 3.0 + (double)slots * s * hd * 8 / 4e6 : 0.0);
+        const double us = waves * (3.0 * (double)((steps + s - 1) / s) + 4.0) + (s > 1 ? 3.0 + s * join_us(slots, hd) : 0.0);
         if (s == 1 || us < least) least = us, best = s;
     }
     return best;
@@ -959,23 +969,33 @@ int64_t attend_parts(const Kv8 &c, int64_t units, int64_t span) {
     return std::min<int64_t>({fill, span / 128, 128});
 }
 
+// The same for float32 rows too: a warp sums every 4th group of 16 positions, and the tensor cores cut sums off towards 0
+// (about 1e-8 a step), so their results are joined from parts of at most 1024 positions.
+int64_t few_parts(const Kv8 &c, int64_t units, int64_t span, int type) {
+    const int64_t want = attend_parts(c, units, span);
+    return type == LLMB_F32 ? std::max<int64_t>(want, (span + 1023) / 1024) : want;
+}
+
 // Whether the kernel for many rows takes the call.  It starts slower and does more for each byte of the cache: below about
 // 2 million (row, query head, position) of 64 elements the kernel for few rows is faster, 2.5 million where rows are two
 // pieces and its tiles 8 rows (B200, us, few / many rows; bfloat16: 1.3 M 14.5 / 16.5, 1.8 M 15.9 / 15.6, 2.2 M 19.0 / 15.3;
 // float32: 1.8 M 16.2 / 17.0, 2.2 M 16.5 / 17.7 and 17.0 / 21.3, 2.6 M 24.1 / 19.6).  A tile of 128 rows with few of them
 // is no gain: a decoding step stays with the other.
+constexpr double few_work(int type) { return type == LLMB_BF16 ? 2e6 : 2.5e6; }
+
 bool many_rows(const Kv8 &c, int heads, int hd, int type, int window) {
     const int64_t seen = window > 0 ? std::min<int64_t>(c.cap, (int64_t)window + c.max_new) : c.cap;
-    return (int64_t)c.max_new * (heads / c.kvh) > 32 &&
-           (double)c.nrows * heads * (double)seen * (hd / 64) > (type == LLMB_BF16 ? 2e6 : 2.5e6);
+    return (int64_t)c.max_new * (heads / c.kvh) > 32 && (double)c.nrows * heads * (double)seen * (hd / 64) > few_work(type);
 }
+
+int few_tile(int64_t rows, int type) { return type == LLMB_BF16 && rows > 8 ? 16 : 8; }
 
 Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
     Cut k{};
     const int group = heads / c.kvh;
     const int64_t rows = (int64_t)c.max_new * group;
     k.chunk = many_rows(c, heads, hd, type, window);
-    const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : type == LLMB_BF16 && rows > 8 ? 16 : 8;
+    const int tile = k.chunk ? kv8_chunk_rows(type == LLMB_F32, hd) : few_tile(rows, type);
     k.tile = tile;
     k.tiles = (int)((rows + tile - 1) / tile);
     // the most positions that a tile's rows see between them
@@ -985,28 +1005,29 @@ Cut attention_cut(const Kv8 &c, int heads, int hd, int type, int window) {
         return std::min<int64_t>(c.cap, (int64_t)w + tokens + 15);
     };
     const int64_t units = (int64_t)c.nseq * c.kvh * std::max(k.tiles, 1);
-    auto parts = [&](int64_t span) -> int64_t {
-        if (k.chunk) return chunk_parts(units, span, (int64_t)c.nrows * heads, hd);
-        int64_t want = attend_parts(c, units, span);
-        // a warp sums every 4th group of 16 positions, and the tensor cores cut sums off towards 0 (about 1e-8 a step):
-        // float32 results are joined from parts of at most 1024 positions
-        if (type == LLMB_F32) want = std::max<int64_t>(want, (span + 1023) / 1024);
-        return want;
-    };
     const int64_t span = span_of(window);
-    const int64_t want = parts(span);
+    const int64_t want = k.chunk ? chunk_parts(units, span, (int64_t)c.nrows * heads, hd) : few_parts(c, units, span, type);
     k.part = (int)((span + want - 1) / want + 127) / 128 * 128;
     k.splits = std::max((int)((span + k.part - 1) / k.part), 1);
     return k;
 }
 
-// The most parts that any window gives, by either kernel: what the workspace has room for.
-int64_t most_parts(const Kv8 &c, int heads, int type) {
-    const int64_t rows = (int64_t)c.max_new * (heads / c.kvh), tile = type == LLMB_BF16 && rows > 8 ? 16 : 8;
-    const int64_t units = (int64_t)c.nseq * c.kvh * std::max<int64_t>((rows + tile - 1) / tile, 1);
-    int64_t most = attend_parts(c, units, c.cap);
-    if (type == LLMB_F32) most = std::max<int64_t>(most, ((int64_t)c.cap + 1023) / 1024);
-    if (rows > 32) most = std::max<int64_t>(most, std::min<int64_t>(64, ((int64_t)c.cap + 127) / 128));
+// The most parts that any type and window give, by either kernel: what the workspace has room for.  Fewer positions are never
+// cut into more parts, and more work never leaves the kernel for many rows.
+int64_t most_parts(const Kv8 &c, int heads, int hd) {
+    const int64_t rows = (int64_t)c.max_new * (heads / c.kvh);
+    auto units = [&](int tile) { return (int64_t)c.nseq * c.kvh * std::max<int64_t>((rows + tile - 1) / tile, 1); };
+    int64_t most = 1;
+    for (int type : {LLMB_F32, LLMB_BF16}) {  // (float16 has the tiles and rules of one or the other)
+        int64_t span = c.cap;
+        if (many_rows(c, heads, hd, type, 0)) {
+            for (bool f32 : {false, true})
+                most = std::max<int64_t>(most, chunk_most_parts(units(kv8_chunk_rows(f32, hd)), c.cap, (int64_t)c.nrows * heads, hd));
+            // the kernel for few rows is left windows with so little work: positions a tile sees, 15 more for a start within 16
+            span = std::min<int64_t>(span, (int64_t)(few_work(type) / ((double)c.nrows * heads * (hd / 64))) + 15);
+        }
+        most = std::max(most, few_parts(c, units(few_tile(rows, type)), span, type));
+    }
     return most;
 }
 
@@ -1065,8 +1086,7 @@ int64_t llmb_kv8_attention_workspace(const llmb_kv8_cache *cache, const llmb_kv8
         op_error(LLMB_ERR_ARG, "llm: kv8_attention_workspace: %d heads on %d kv heads", heads, c.kvh);
         return -1;
     }
-    int64_t splits = 1;
-    for (int type : {LLMB_F32, LLMB_BF16}) splits = std::max(splits, most_parts(c, heads, type));
+    const int64_t splits = most_parts(c, heads, cache->head_dim);
     return splits == 1 ? 0 : (int64_t)c.nrows * heads * splits * (8 + 4 * (int64_t)cache->head_dim);
 }
 
@@ -1084,23 +1104,24 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
         return op_error(LLMB_ERR_ARG, "llm: %s: window %d, scale %g", what, window, (double)scale);
     if ((rc = kv8_rows(what, type, q_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
     if ((rc = kv8_rows(what, type, out_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
-    int dev = 0;
-    if ((rc = kv8_pointers(what, &dev, c, q, "q", out, "out", c.nrows == 0)) != LLMB_OK) return rc;
-    if (c.max_new == 0) return LLMB_OK;
     Kv8Att a{};
     const Cut cut = attention_cut(c, heads, hd, type, window);
     if ((int64_t)c.kvh * cut.tiles > 65535 || (int64_t)c.max_new * heads > INT32_MAX)
         return op_error(LLMB_ERR_ARG, "llm: %s: %d rows of a sequence are too many", what, c.max_new);
-    const int64_t slots = (int64_t)c.nrows * heads * cut.splits;
-    if (cut.splits > 1) {
-        const std::initializer_list<OpPointer> ps = {{workspace, "workspace", 16, false}};
-        if ((rc = op_alignment(what, ps)) != LLMB_OK || (rc = op_pointers(what, dev, ps)) != LLMB_OK) return rc;
+    const int64_t slots = c.max_new > 0 && cut.splits > 1 ? (int64_t)c.nrows * heads * cut.splits : 0;
+    const std::initializer_list<OpPointer> ws = {{workspace, "workspace", 16, slots == 0}};
+    if (slots > 0) {
+        if ((rc = op_alignment(what, ws)) != LLMB_OK) return rc;
         if (workspace_bytes < slots * (8 + 4 * (int64_t)hd))
-            return op_error(LLMB_ERR_ARG, "llm: %s: a workspace of %lld bytes (llmb_kv8_attention_workspace says %lld)",
-                            what, (long long)workspace_bytes, (long long)(slots * (8 + 4 * (int64_t)hd)));
+            return op_error(LLMB_ERR_ARG, "llm: %s: a workspace of %lld bytes, not %lld", what, (long long)workspace_bytes,
+                            (long long)(slots * (8 + 4 * (int64_t)hd)));
         a.part_o = static_cast<float *>(workspace);
         a.part_ml = reinterpret_cast<float2 *>(a.part_o + slots * hd);
     }
+    int dev = 0;
+    if ((rc = kv8_pointers(what, &dev, c, q, "q", out, "out", c.nrows == 0)) != LLMB_OK) return rc;
+    if (slots > 0 && (rc = op_pointers(what, dev, ws)) != LLMB_OK) return rc;
+    if (c.max_new == 0) return LLMB_OK;
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.heads = heads, a.group = heads / c.kvh, a.window = window;
     a.scale = (float)((scale != 0.f ? (double)scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);

@@ -3,11 +3,14 @@
 Helpers, the plain restatement and the tolerances are test_kv8.py's.
 """
 
+import ctypes as C
 import math
+import random
 
 import numpy as np
 import pytest
 
+import llm_b200
 from tests.test_kv8 import DTYPES, Device, _filled, _reference_by_head, _rows, _t, _tolerance, _workspace
 
 gpu = pytest.mark.gpu
@@ -147,3 +150,48 @@ def test_windows_up_to_the_largest_integer(window, lens, new, heads, dtype):
         whole, _, _ = _attention(d, lens, new, heads, dtype, q)
         # (another window may cut the positions into other parts: two results within their tolerance)
         assert ((got - whole).abs() <= 2 * tol).all() and (got[:new[0] - lens[0]] == 0).all()
+
+
+# ---------------------------------------------------------------- the workspace's size, without a GPU
+
+
+def _need(c, b, heads, type_, window, said):
+    """Whether the call accepts a workspace of that many bytes (what comes after that check fails here: no memory of a
+    GPU)."""
+    L = llm_b200.lib()
+    cache = C.cast(c, C.POINTER(llm_b200._KV8Cache)).contents
+    width = heads * cache.head_dim
+    assert L.llmb_kv8_attention(c, b, 4096, width, 4096, width, type_, heads, 0.0, window, 4096, said, None) != llm_b200.OK
+    return b"a workspace of" not in L.llmb_last_error(None)
+
+
+def _sizes(seqs, rows, max_new, max_len, kv, hd, block=64):
+    c = llm_b200._KV8Cache(4096, 8192, 256, 512, kv * block * hd, 8, block, kv, hd, 0)
+    return C.byref(c), C.byref(llm_b200._KV8Batch(256, 512, 1024, seqs, -(-max_len // block), rows, max_new, max_len))
+
+
+@pytest.mark.parametrize("seqs,rows,max_new,max_len,at_most", [(3, 2563, 1023, 5000, 200 << 20), (1, 8192, 8192, 8192, 300 << 20),
+                                                               (16, 16 * 4096, 4096, 4096, 0), (64, 64 * 4096, 4096, 4096, 0)])
+def test_the_workspace_of_prompts_is_what_their_cut_can_need(seqs, rows, max_new, max_len, at_most):
+    """32 heads on 8 of size 128.  (An attention's own output for 64 prompts of 4096 is 2 GiB in bfloat16.)"""
+    c, b = _sizes(seqs, rows, max_new, max_len, 8, 128)
+    said = llm_b200.lib().llmb_kv8_attention_workspace(c, b, 32)
+    assert 0 <= said <= at_most
+
+
+def test_no_call_needs_more_workspace_than_is_said():
+    rng = random.Random(1)
+    split = 0
+    for _ in range(1500):
+        kv, group, hd = rng.choice([1, 2, 3, 8]), rng.choice([1, 3, 4, 7, 64]), rng.choice([64, 128])
+        seqs, max_new = int(2 ** rng.uniform(0, 8)), int(2 ** rng.uniform(0, 13))
+        rows = rng.randint(max_new, max_new * seqs)
+        max_len = int(2 ** rng.uniform(0, 20))
+        c, b = _sizes(seqs, rows, max_new, max_len, kv, hd)
+        said = llm_b200.lib().llmb_kv8_attention_workspace(c, b, kv * group)
+        assert said >= 0
+        for window in [0] + [int(2 ** rng.uniform(0, 20)) for _ in range(6)]:
+            for type_ in range(3):
+                assert _need(c, b, kv * group, type_, window, said), (seqs, rows, max_new, max_len, kv, group, hd, window, type_)
+                split += not _need(c, b, kv * group, type_, window, 0)
+    assert split > 5000  # (many of the calls are cut)
