@@ -407,22 +407,36 @@ def _flat(t, what: str, name: str, shape: tuple) -> int:
     return t.data_ptr()
 
 
+def _int32(what: str, v: int) -> int:
+    """v, which the C structures hold in 32 bits."""
+    if not -1 << 31 <= v < 1 << 31:
+        _refuse(f"{what} {v} out of range")
+    return v
+
+
 class KV8Batch:
     """The sequences of one call on a KV8Cache (llmb_kv8_batch): lens [n_seq] positions each holds once this call's
     rows are in, tables [n_seq, entries] its block numbers, starts [n_seq + 1] where its rows begin (None: rows / n_seq
     each), all int32 on the device. The tensors' contents may change between calls; max_new and max_len (0: not known)
-    bound the rows and the positions of any one sequence."""
+    bound the rows and the positions of any one sequence. A batch of other sizes is another KV8Batch."""
 
     def __init__(self, lens, tables, starts=None, rows: int = 0, max_new: int = 0, max_len: int = 0):
         if len(tables.shape) != 2 or len(lens.shape) != 1 or tables.shape[0] != lens.shape[0]:
             _refuse("lens must be [n_seq], tables [n_seq, entries]")
         n, entries = lens.shape[0], tables.shape[1]
         self._keep = (lens, tables, starts)
-        self.rows = rows
+        for what, x in (("rows", rows), ("max_new", max_new), ("max_len", max_len), ("table entries", entries)):
+            _int32(what, x)
         self._c = _KV8Batch(_flat(lens, "lens", "int32", (n,)), _flat(tables, "tables", "int32", (n, entries)),
                             None if starts is None else _flat(starts, "starts", "int32", (n + 1,)),
                             n, entries, rows, max_new, max_len)
         self._at = C.addressof(self._c)
+        self._n_rows = rows  # (kept beside the structure: a look into that costs more)
+
+    @property
+    def rows(self) -> int:
+        """Rows of the calls' tensors; the kernels go by the same number."""
+        return self._n_rows
 
 
 class KV8Cache:
@@ -442,24 +456,32 @@ class KV8Cache:
                 _refuse("k and v must be contiguous within a block and have one block stride")
         scales = [_flat(x, "a scale", "float32", (n, heads)) for x in (k_scale, v_scale)]
         self._keep = (k, v, k_scale, v_scale)
-        self.kv_heads, self.head_dim = heads, hd
+        self._kv_heads, self._head_dim = heads, hd
         self._c = _KV8Cache(k.data_ptr(), v.data_ptr(), *scales,
                             max(k.stride(0), heads * block * hd) if n == 1 else k.stride(0), n, block, heads, hd,
                             KV8_INT8 if t == 10 else KV8_E4M3)
         self._at = C.addressof(self._c)
         self._rows, self._attend = _calls().rows, _calls().attention
 
+    @property
+    def kv_heads(self) -> int:
+        return self._kv_heads
+
+    @property
+    def head_dim(self) -> int:
+        return self._head_dim
+
     def append(self, batch: KV8Batch, k, v, stream: int = 0) -> None:
         """Writes the rows k, v [rows, kv_heads, head_dim] (llmb_kv8_append)."""
-        self._rows(0, self._at, batch._at, batch.rows, self.kv_heads, self.head_dim, k, v, stream)
+        self._rows(0, self._at, batch._at, batch._n_rows, self._kv_heads, self._head_dim, k, v, stream)
 
     def read(self, batch: KV8Batch, k=None, v=None, stream: int = 0) -> None:
         """Reads what is held at the rows' positions into k, v [rows, kv_heads, head_dim] (llmb_kv8_read)."""
-        self._rows(1, self._at, batch._at, batch.rows, self.kv_heads, self.head_dim, k, v, stream)
+        self._rows(1, self._at, batch._at, batch._n_rows, self._kv_heads, self._head_dim, k, v, stream)
 
     def attention_workspace(self, batch: KV8Batch, heads: int) -> int:
         """Bytes of workspace for attention() with that many query heads (llmb_kv8_attention_workspace)."""
-        n = lib().llmb_kv8_attention_workspace(C.byref(self._c), C.byref(batch._c), heads)
+        n = lib().llmb_kv8_attention_workspace(C.byref(self._c), C.byref(batch._c), _int32("heads", heads))
         if n < 0:
             _op_check(ERR_ARG)
         return n
@@ -468,7 +490,7 @@ class KV8Cache:
                   stream: int = 0) -> None:
         """Attention of the queries q [rows, heads, head_dim] over the cache into out (llmb_kv8_attention); workspace:
         a contiguous tensor of attention_workspace() bytes."""
-        self._attend(self._at, batch._at, batch.rows, self.head_dim, q, out, scale, window, workspace, stream)
+        self._attend(self._at, batch._at, batch._n_rows, self._head_dim, q, out, scale, window, workspace, stream)
 
 
 def logits_control(logits, out=None, tokens=None, history=None, history_lens=None, prompt_lens=None, penalties=None,

@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 
 import llm_b200
+from llm_b200 import LlmError
 from tests.test_kv8 import DTYPES, Device, _filled, _reference_by_head, _rows, _t, _tolerance, _workspace
 
 gpu = pytest.mark.gpu
@@ -195,3 +196,37 @@ def test_no_call_needs_more_workspace_than_is_said():
                 assert _need(c, b, kv * group, type_, window, said), (seqs, rows, max_new, max_len, kv, group, hd, window, type_)
                 split += not _need(c, b, kv * group, type_, window, 0)
     assert split > 5000  # (many of the calls are cut)
+
+
+# ---------------------------------------------------------------- the Python objects, without a GPU
+
+
+def _objects():
+    torch, _, _ = _t()
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.int8)
+    s = torch.ones(4, 2)
+    lens, tables = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    return llm_b200.KV8Cache(k, k, s, s), lens, tables
+
+
+def test_sizes_that_the_kernels_go_by_cannot_be_changed():
+    """What the tensors are checked against is what the C structures hold."""
+    torch, _, _ = _t()
+    cache, lens, tables = _objects()
+    batch = llm_b200.KV8Batch(lens, tables, rows=2)
+    assert (batch.rows, cache.kv_heads, cache.head_dim) == (2, 2, 64)
+    for o, name in ((batch, "rows"), (cache, "kv_heads"), (cache, "head_dim")):
+        with pytest.raises(AttributeError):
+            setattr(o, name, 1)
+    x = torch.zeros(1, 2, 64)
+    with pytest.raises(LlmError):
+        cache.append(batch, x, x)
+
+
+def test_sizes_past_32_bits_are_refused():
+    cache, lens, tables = _objects()
+    for kw in (dict(rows=1 << 32), dict(rows=2, max_new=(1 << 32) + 1), dict(rows=2, max_len=1 << 31), dict(rows=-(1 << 40))):
+        with pytest.raises(LlmError, match="out of range"):
+            llm_b200.KV8Batch(lens, tables, **kw)
+    with pytest.raises(LlmError, match="out of range"):
+        cache.attention_workspace(llm_b200.KV8Batch(lens, tables, rows=2), (1 << 32) + 14)
