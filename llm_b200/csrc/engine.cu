@@ -1015,6 +1015,10 @@ Error generate_controlled(Model &m, const int32_t *prompt, int np, int n, int32_
         m.stats.tokens++;
         if (emit && !emit(user, tok)) break;
     }
+    if (tm.prefill_ms == 0) {  // stopped before the first token
+        CUDA_TRY(cudaStreamSynchronize(m.st));
+        tm.prefill_ms = now_ms() - t0, t1 = now_ms();
+    }
     CUDA_TRY(cudaEventRecord(m.ev3, m.st));
     CUDA_TRY(cudaEventSynchronize(m.ev3));  // (a launch that a stop left behind, too)
     if ((err = check_device(m)).code) return err;
