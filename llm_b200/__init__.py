@@ -315,8 +315,14 @@ class GPU:
 
         mask_fn, emit_fn = MASK_FN(), EMIT_FN()
         if mask is not None:
-            mask_fn = MASK_FN(guarded(lambda _u, t, k, w: mask(
-                np.ctypeslib.as_array(t, (k,)).copy() if k else np.zeros(0, np.int32), np.ctypeslib.as_array(w, (words,)))))
+            allowed = np.zeros(words, np.uint32)  # the callback's to keep: the library's own words end with the model
+
+            def fill(_u, t, k, w):
+                go = mask(np.ctypeslib.as_array(t, (k,)).copy() if k else np.zeros(0, np.int32), allowed)
+                C.memmove(w, allowed.ctypes.data, allowed.nbytes)
+                return go
+
+            mask_fn = MASK_FN(guarded(fill))
         if emit is not None:
             emit_fn = EMIT_FN(guarded(lambda _u, t: emit(int(t))))
         c = _Controls(repetition, presence, frequency, len(ids), ids.ctypes.data, values.ctypes.data, mask_fn, None)
