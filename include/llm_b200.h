@@ -382,7 +382,8 @@ typedef struct {
 
 /* llmb_generate with llmb_logits_control between the model's logits and each
  * token (the prompt and the answer so far are the history).  Stops as
- * Generate does, and where no token is allowed.  One token per launch, each
+ * Generate does, and where no token is allowed.  With penalties the prompt and
+ * n are at most 524288 tokens together.  One token per launch, each
  * read back before the next. */
 LLMB_API int llmb_generate_controlled(llmb_model *m, const int32_t *prompt, int n_prompt, int n, int32_t eos,
                                       const llmb_controls *controls, llmb_emit_fn emit, void *user,

@@ -932,6 +932,8 @@ Error generate_logits(Model &m, const int32_t *prompt, int np, int n, int32_t *t
     return err;
 }
 
+constexpr int kMaxHistory = 524287;  // llmb_logits_ctl's history_stride
+
 // What llmb_logits_control reads on the device, followed by the mask's words.
 struct ControlBuffer {
     float penalties[3];
@@ -963,6 +965,11 @@ Error generate_controlled(Model &m, const int32_t *prompt, int np, int n, int32_
     for (int i = 0; i < ctl->n_bias; i++)
         if (ctl->bias_ids[i] < 0 || ctl->bias_ids[i] >= m.cfg.vocab || std::isnan(ctl->bias_values[i]))
             return {LLMB_ERR_ARG, "llm: bias " + std::to_string(i) + " is NaN or of no token"};
+    // (penalties that do nothing need no history)
+    const bool penalised = ctl->repetition != 1.f || ctl->presence != 0.f || ctl->frequency != 0.f;
+    if (penalised && (int64_t)np + n - 1 > kMaxHistory)
+        return {LLMB_ERR_CONTEXT, "llm: penalties over a prompt of " + std::to_string(np) + " tokens and " + std::to_string(n) +
+                                      " new ones (at most " + std::to_string(kMaxHistory + 1) + " together)"};
     const size_t words = ((size_t)m.cfg.vocab + 31) / 32, bytes = sizeof(ControlBuffer) + words * 4;
     if (!m.ctl && !(m.ctl = m.alloc<uint8_t>(bytes, err))) return err;
     if (!m.h_ctl) CUDA_TRY(cudaHostAlloc(&m.h_ctl, bytes, cudaHostAllocDefault));
@@ -995,7 +1002,8 @@ Error generate_controlled(Model &m, const int32_t *prompt, int np, int n, int32_
         if (ctl->mask && !ctl->mask(ctl->mask_user, tokens.data(), (int)tokens.size(), h_mask)) break;
         if (ctl->mask) CUDA_TRY(cudaMemcpyAsync(d_mask, h_mask, words * 4, cudaMemcpyHostToDevice, m.st));
         llmb_logits_ctl c{};
-        c.history = m.hdm.tokens, c.history_stride = np + i, c.prompt_lens = &d.prompt_len, c.penalties = d.penalties;
+        if (penalised)
+            c.history = m.hdm.tokens, c.history_stride = np + i, c.prompt_lens = &d.prompt_len, c.penalties = d.penalties;
         if (ctl->n_bias > 0) c.n_bias = ctl->n_bias, c.bias_ids = d.bias_ids, c.bias_values = d.bias_values;
         if (ctl->mask) c.mask = d_mask, c.mask_stride = (int32_t)words;
         const int rc = llmb_logits_control(m.hdm.logits, m.cfg.vocab, LLMB_F32, 1, m.cfg.vocab, &c, nullptr, 0,
