@@ -265,8 +265,9 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8 c, T *__restrict__ k
     const Kv8Seq q = kv8_seq(c, s);
     if (q.n <= 0) return;
     // blocks counted from the one that holds the first row's position, which may be below 0
-    const int j = (q.first >> c.bshift) + (int)blockIdx.x, p0 = j * c.block, end = q.first + q.n;
-    if (p0 >= end) return;
+    const int j = (q.first >> c.bshift) + (int)blockIdx.x, end = q.first + q.n;
+    if ((int64_t)j * c.block >= end) return;  // (a longer sequence's blocks, counted from the largest length, pass 2^31)
+    const int p0 = j * c.block;
     const int b = kv8_block(c, s, j);
     const int lo = max(q.first - p0, 0), hi = min(end - p0, c.block);
     // the threads take 256 / per tiles at once, or a tile in per / 256 steps (both powers of two)

@@ -230,3 +230,21 @@ def test_sizes_past_32_bits_are_refused():
             llm_b200.KV8Batch(lens, tables, **kw)
     with pytest.raises(LlmError, match="out of range"):
         cache.attention_workspace(llm_b200.KV8Batch(lens, tables, rows=2), (1 << 32) + 14)
+
+
+@gpu
+def test_the_largest_length_beside_a_long_sequence():
+    """A length of 2^31 - 1 in a batch with a sequence of many rows: its rows are 0 (no table reaches there), and no other
+    row is written, nor any byte of the cache."""
+    torch, _, _ = _t()
+    rng = np.random.default_rng(26)
+    d = _filled(2, 16, 64, "int8", [100, 100], rng)
+    before = d.k.clone(), d.v.clone(), d.ks.clone(), d.vs.clone()
+    m = 40000
+    batch = d.batch([2 ** 31 - 1, -1], [3, m], rows=m + 5)
+    k = torch.full((m + 5, 2, 64), 5.0, device="cuda")
+    d.cache.append(batch, k, k)
+    d.cache.read(batch, k)
+    assert (k[:m + 3] == 0).all() and (k[m + 3:] == 5).all()
+    for a, b in zip(before, (d.k, d.v, d.ks, d.vs)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
