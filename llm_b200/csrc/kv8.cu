@@ -1105,6 +1105,8 @@ int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch,
         return op_error(LLMB_ERR_ARG, "llm: %s: window %d, scale %g", what, window, (double)scale);
     if ((rc = kv8_rows(what, type, q_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
     if ((rc = kv8_rows(what, type, out_stride, (int64_t)heads * hd)) != LLMB_OK) return rc;
+    if (out == q && c.nrows > 1 && out_stride != q_stride)
+        return op_error(LLMB_ERR_ARG, "llm: %s: out is q with another stride", what);
     Kv8Att a{};
     const Cut cut = attention_cut(c, heads, hd, type, window);
     if ((int64_t)c.kvh * cut.tiles > 65535 || (int64_t)c.max_new * heads > INT32_MAX)

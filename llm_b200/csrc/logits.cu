@@ -297,6 +297,8 @@ extern "C" int llmb_logits_control(const void *logits, int64_t stride, int type,
     if (rows < 0 || rows > 65535 || vocab < 1 || vocab > 1 << 24 || stride < vocab || (out && out_stride < vocab))
         return op_error(LLMB_ERR_ARG, "llm: %s: %d rows of %d logits, %lld and %lld elements apart", what, rows, vocab,
                         (long long)stride, (long long)out_stride);
+    if (out == logits && rows > 1 && out_stride != stride)
+        return op_error(LLMB_ERR_ARG, "llm: %s: out is logits with another stride", what);
     if (!out && !tokens && rows > 0) return op_error(LLMB_ERR_ARG, "llm: %s: neither out nor tokens", what);
     if (ctl->history && (ctl->history_stride < 1 || ctl->history_stride > kMaxHistory))
         return op_error(LLMB_ERR_ARG, "llm: %s: histories of %d tokens (1 to %d)", what, ctl->history_stride, kMaxHistory);

@@ -248,3 +248,16 @@ def test_the_largest_length_beside_a_long_sequence():
     assert (k[:m + 3] == 0).all() and (k[m + 3:] == 5).all()
     for a, b in zip(before, (d.k, d.v, d.ks, d.vs)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_in_place_with_another_stride_is_refused():
+    """Rows would be overwritten before others have read them."""
+    L, arg = llm_b200.lib(), llm_b200.ERR_ARG
+    c, b = _sizes(2, 4, 2, 100, 2, 64)
+    for q_stride, out_stride, refused in ((512, 256, True), (256, 512, True), (256, 256, False)):
+        rc = L.llmb_kv8_attention(c, b, 4096, q_stride, 4096, out_stride, 0, 4, 0.0, 0, 4096, 1 << 30, None)
+        assert rc != llm_b200.OK and (b"another stride" in L.llmb_last_error(None)) == refused
+        ctl = llm_b200._LogitsCtl()
+        rc = L.llmb_logits_control(4096, q_stride, 0, 2, 200, C.byref(ctl), 4096, out_stride, 256, None)
+        assert rc != llm_b200.OK and (b"another stride" in L.llmb_last_error(None)) == refused
+        assert not refused or rc == arg
