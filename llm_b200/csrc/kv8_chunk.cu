@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                     }
                     if (fresh) {
                         raise(find());
+                        tm_st_wait();  // (stores of one thread have no order of their own)
                         sum = weigh(big);
                     }
                 } else {  // (two pieces leave no registers for weighing twice: 232 us for 194)
