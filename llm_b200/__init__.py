@@ -400,7 +400,8 @@ def _calls():
         try:
             module = importlib.import_module("._native", __name__)
         except ImportError as e:
-            raise ImportError(f"{e}: build it with `python -m llm_b200.build`") from e
+            raise ImportError(f"{e}: build it with `python -m llm_b200.build` (a C compiler and Python 3.12 or later "
+                              "with its headers)") from e
         module.setup(_TYPES, _refuse, _op_check)
         _native_calls = module
     return _native_calls

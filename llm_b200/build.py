@@ -1,5 +1,7 @@
 """Builds llm_b200/libllmb200.so with nvcc for sm_100a, and _native.abi3.so, the Python calls of its operators (in-tree, so
-that they travel with the repository).
+that they travel with the repository). The latter needs a C compiler ($CC or gcc) and the headers of Python 3.12 or later;
+without them it is left out, with a note: the library and the rest of the package do not need it, KV8Cache and
+logits_control raise ImportError.
 
     python -m llm_b200.build          # incremental
     python -m llm_b200.build --force  # rebuild everything
@@ -8,6 +10,7 @@ that they travel with the repository).
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -34,6 +37,18 @@ def _nvcc() -> str:
     return "nvcc"
 
 
+def _no_calls() -> str:
+    """Why the Python calls of the operators cannot be built here ("": they can)."""
+    cc = os.environ.get("CC", "gcc").split()
+    if not cc or not shutil.which(cc[0]):
+        return f"no C compiler {' '.join(cc)!r}"
+    if sys.version_info < (3, 12):
+        return "Python 3.12 or later is needed"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "no Python.h"
+    return ""
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     hdr_mtime = max([os.path.getmtime(os.path.join(CSRC, h)) for h in HEADERS] + [os.path.getmtime(__file__)])
@@ -55,9 +70,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
         os.replace(tmp, LIB)
     src = os.path.join(CSRC, "call.c")
     header = os.path.join(ROOT, "include", "llm_b200.h")
-    if force or not os.path.exists(CALL) or os.path.getmtime(CALL) < max(os.path.getmtime(f) for f in (src, header, __file__)):
+    why = _no_calls()
+    if why:
+        print(f"llm_b200: built without the Python calls of the operators: {why}", file=sys.stderr)
+    elif force or not os.path.exists(CALL) or os.path.getmtime(CALL) < max(os.path.getmtime(f) for f in (src, header, __file__)):
         tmp = CALL + ".tmp"
-        subprocess.run([os.environ.get("CC", "gcc"), "-O2", "-std=c11", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
+        subprocess.run([*os.environ.get("CC", "gcc").split(), "-O2", "-std=c11", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
                         "-I", sysconfig.get_paths()["include"], src, "-o", tmp, "-L", HERE, "-l:libllmb200.so",
                         "-Wl,-rpath,$ORIGIN"], check=True)
         os.replace(tmp, CALL)
