@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libllmb200.so")
 CALL = os.path.join(HERE, "_native.abi3.so")
 SOURCES = ["gguf.cpp", "kernels.cu", "gemm.cu", "decode.cu", "engine.cu", "noalloc.cu", "ops.cpp", "kv8.cu", "kv8_chunk.cu", "logits.cu"]
-HEADERS = ["gguf.hpp", "device.hpp", "kernels.hpp", "ops.hpp", "kv8.hpp", "kv8_chunk.hpp", os.path.join("..", "..", "include", "llm_b200.h")]
+HEADERS = ["gguf.hpp", "device.hpp", "kernels.hpp", "ops.hpp", "ptx.hpp", "kv8.hpp", "kv8_chunk.hpp", os.path.join("..", "..", "include", "llm_b200.h")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", os.path.join(ROOT, "include")]
 # The persistent decode kernel's launch bounds still set its register budget; with this flag ptxas allocates

@@ -12,11 +12,10 @@
 #include "kv8.hpp"
 #include "kv8_chunk.hpp"
 #include "ops.hpp"
+#include "ptx.hpp"
 
 namespace llmb {
 namespace {
-
-constexpr unsigned kFull = 0xffffffffu;
 
 // ------------------------------------------------------------- append --
 
@@ -338,11 +337,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // What 16 positions share: where they lie in the pools (below 0: nowhere), K's scale, V's scale = mv 2^lv with 2^-lv.
 struct Place {
     int64_t at;
@@ -393,10 +387,10 @@ __host__ __device__ constexpr int att_groups(int hd, int nb) { return hd == 64 &
 __host__ __device__ constexpr int att_smem(int hd) { return kAttWarps * att_depth(hd) * 32 * hd; }
 
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(su32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp8(void *dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(su32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

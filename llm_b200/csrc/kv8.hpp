@@ -10,6 +10,7 @@
 
 namespace llmb {
 
+constexpr unsigned kFull = 0xffffffffu;
 constexpr int kKv8MaxLen = 0x7fffffff - 16384;  // sums of positions and a block, a step or a set of them stay below 2^31
 
 // The cache and the batch of a call as the kernels take them (include/llm_b200.h describes the fields).
@@ -72,6 +73,11 @@ __device__ __forceinline__ __half kv8_from<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 kv8_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // Two 8-bit values as float16, exactly.  w holds them in its bytes 0 and 2
 // (E4M3: times 2^-8, and bytes that are NaN come out finite, so that no byte
 // of a masked position can make a product NaN).
@@ -128,7 +134,7 @@ __device__ __forceinline__ int kv8_v_scale(float vs, float &mv, int &low) {
     const uint32_t u = __float_as_uint(vs) & 0x7fffffffu;
     const bool has = u >= (uint32_t)(127 + kKv8LeastScale) << 23 && u < 0x7f800000u;
     int ex = has ? min(max((int)(u >> 23) - 127, kKv8LeastExp), 126) : kKv8NoExp;
-    low = min(low, __reduce_min_sync(0xffffffffu, ex));
+    low = min(low, __reduce_min_sync(kFull, ex));
     if (!has) ex = low == kKv8NoExp ? kKv8ZeroExp : low;
     mv = vs * kv8_pow2(-ex);
     return ex;

@@ -45,11 +45,11 @@
 #include "kv8.hpp"
 #include "kv8_chunk.hpp"
 #include "ops.hpp"
+#include "ptx.hpp"
 
 namespace llmb {
 namespace {
 
-constexpr unsigned kFull = 0xffffffffu;
 constexpr int kKeys = 128;                  // positions of a step
 constexpr int kThreads = 16 * 32;           // warpgroups: A's softmax, B's softmax, the converters, the issuer and the copier
 // Their registers a thread: as many together as the launch's 4 x 128.
@@ -96,24 +96,6 @@ struct Bars {
     uint32_t tmem, fail, none[8];  // none: a step's groups whose values are 0, a bit each
 };
 static_assert(sizeof(Bars) <= 384, "the barriers' space");
-
-__device__ __forceinline__ uint32_t su32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(su32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ uint64_t gtime() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 
 // Waits for a phase of a barrier, at most kWaitNs (counted from the first look at the clock, which is slow and so left
 // until many tries were in vain); false after that, or once another wait has run out.
@@ -219,11 +201,6 @@ __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;

@@ -35,13 +35,13 @@
 
 #include "kv8.hpp"
 #include "ops.hpp"
+#include "ptx.hpp"
 
 namespace llmb {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 384;
 constexpr int kMaxSlice = 11264;  // tokens of a CTA and round: a table of 44 KiB
 constexpr int kMaxBias = 4095, kMaxHistory = (1 << 19) - 1;
@@ -66,8 +66,6 @@ __device__ __forceinline__ uint64_t rank_of(float x, int v) {
     const uint32_t key = u & 0x80000000u ? ~u : u | 0x80000000u;
     return (uint64_t)key << 32 | (uint32_t)~v;
 }
-
-__device__ __forceinline__ uint32_t su32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) k_logits(const Ctl c) {
