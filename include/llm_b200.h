@@ -311,15 +311,22 @@ LLMB_API int llmb_kv8_read(const llmb_kv8_cache *cache, const llmb_kv8_batch *ba
  * n_rows rows of [heads][head_dim] elements of `type`, q_stride and
  * out_stride elements apart, 16-byte aligned; out must not overlap q unless
  * it is the same buffer with the same stride.  scale 0 means
- * 1 / sqrt(head_dim), negative ones are refused.  A row that sees no position becomes 0, one whose query
- * is not finite NaN; rows of no sequence stay as they were.  Positions whose
- * block is not in the pool are not seen; a byte that is a NaN of e4m3 (append
- * writes none) is no value of the cache.  (A wait inside the kernel that runs
- * out after 1 s, which only a fault of the GPU can cause, makes the rows NaN.)
- * `workspace`:
- * llmb_kv8_attention_workspace bytes of the caller's, 16-byte aligned, not
- * read before it is written; calls that may overlap on the GPU need their
- * own.  heads / kv_heads at most 64. */
+ * 1 / sqrt(head_dim), negative ones are refused.  A row that sees no position
+ * becomes 0, another whose query is not finite NaN; rows of no sequence stay
+ * as they were.  Positions whose block is not in the pool are not seen.
+ * Blocks' scales are finite and not negative; positions of a block whose
+ * v_scale is 0 count in the softmax and add nothing to the result (a scale
+ * below 2^-109, which append does not make, may be taken as 0).  A byte that
+ * is a NaN of e4m3 (append writes none) is no value of the cache.  (A wait
+ * inside the kernel that runs out after 1 s, which only a fault of the GPU can
+ * cause, makes the rows NaN.)
+ * Precision: 8-bit values enter the products exactly.  float32 queries have
+ * 22 bits of their row's largest element, the weights of float32 and float16
+ * rows 22 bits, those of bfloat16 rows 11 (off by 2^-12, a sixteenth of the
+ * result's own rounding); sums are float32.
+ * `workspace`: llmb_kv8_attention_workspace bytes of the caller's, 16-byte
+ * aligned, not read before it is written; calls that may overlap on the GPU
+ * need their own.  heads / kv_heads at most 64. */
 LLMB_API int llmb_kv8_attention(const llmb_kv8_cache *cache, const llmb_kv8_batch *batch, const void *q,
                                 int64_t q_stride, void *out, int64_t out_stride, int type, int heads, float scale,
                                 int window, void *workspace, int64_t workspace_bytes, void *stream);
@@ -383,8 +390,8 @@ typedef struct {
 /* llmb_generate with llmb_logits_control between the model's logits and each
  * token (the prompt and the answer so far are the history).  Stops as
  * Generate does, and where no token is allowed.  With penalties the prompt and
- * n are at most 524288 tokens together.  One token per launch, each
- * read back before the next. */
+ * n are at most 524288 tokens together.  One token per launch, each read back
+ * before the next. */
 LLMB_API int llmb_generate_controlled(llmb_model *m, const int32_t *prompt, int n_prompt, int n, int32_t eos,
                                       const llmb_controls *controls, llmb_emit_fn emit, void *user,
                                       int32_t *out_tokens, int *n_out, llmb_timing *tm);

@@ -362,19 +362,24 @@ struct Place {
 // Bound, B200: one sequence of 131071 positions (32 heads on 8, size 128,
 // e4m3, bfloat16 rows) 66 us with its join, 4.1 TB/s, 63 % of the measured copy
 // rate: copies in flight and the ends of the one wave.  64 sequences of up to
-// 2048 (9 heads on 3, size 64, int8, float32) 17 us, 1.9 TB/s: 324 instructions
-// a group and the sequences' different lengths; two groups at once save
-// nothing.  300 positions of one sequence 6 us: latency.
+// 2048 (9 heads on 3, size 64, int8, float32) 16.5 us, 2.0 TB/s: 324
+// instructions a group and the sequences' different lengths.  300 positions of
+// one sequence 6 us: latency.
 //
 // float32 rows (PIECES = 2) are the sum of two float16 pieces, which hold 22
 // bits of the row's largest element after a power of two has brought it to
 // [2^14, 2^15); the weights go into the second product the same way.
 // float16 rows fit one piece, but a weight rounded to float16 is off as much
-// as the result's own rounding, so they take the two-piece form as well.
+// as the result's own rounding (2^-12 and 2^-11 relative), so they take the
+// two-piece form as well.  bfloat16 rows and their weights are one piece: a
+// weight is off by 2^-12 at most, a sixteenth of the result's own rounding
+// (2^-8), and the weights' errors are independent, so that a mean over many
+// positions is off by less.  exp2 is the machine's approximation (2^-22
+// relative).
 //
 // The scale of V's block enters the weights' exponent (its power of two, so
 // that the largest weight of all stays near 2^6 and float16 holds the small
-// ones) and mantissa.
+// ones) and mantissa (kv8_v_scale).
 template <class T>
 constexpr int kPieces = 2;
 template <>
@@ -382,7 +387,8 @@ constexpr int kPieces<__nv_bfloat16> = 1;
 
 // Groups of a warp in flight, as many as four CTAs an SM have room for (a group is 32 HD bytes), and their bytes.
 __host__ __device__ constexpr int att_depth(int hd) { return hd == 64 ? 6 : 3; }
-// Groups worked on at once: two where the registers of four CTAs an SM hold them.
+// Groups worked on at once: two where the registers of four CTAs an SM hold them (us, with one / with two: 64 sequences 16.6 /
+// 16.4, the window of 4000 in bfloat16 15.4 / 14.8, a chunk of 64 behind 1920 17.0 / 16.4).
 __host__ __device__ constexpr int att_groups(int hd, int nb) { return hd == 64 && nb == 1 ? 2 : 1; }
 __host__ __device__ constexpr int att_smem(int hd) { return kAttWarps * att_depth(hd) * 32 * hd; }
 

@@ -23,12 +23,13 @@
 // a step's maximum otherwise).
 //
 // Three prompts of up to 1023 tokens behind 4000 positions (32 heads on 8, size
-// 128, int8, bfloat16 rows): 298 us, 637 TFLOP/s, 39 % of the measured bf16
-// rate; 360 tiles are 2.4 waves.  The chain of one tile, softmax and then its
-// two products, bounds a step (without the weights 222 us, without the
-// exponentials 289, without the conversion 316 of 332), then shared memory's
+// 128, int8): bfloat16 rows 300 us, 634 TFLOP/s, 38 % of the measured bf16
+// rate, float16 437, float32 708; 360 tiles are 2.4 waves.  The chain of one
+// tile, softmax and then its two products, bounds a step, then shared memory's
 // rate: 192 KB of operands, 64 KB of float16 stored and 64 KB of copies a step
-// of two tiles.
+// of two tiles.  Left out one at a time, when a step's maximum was still looked
+// for in every step (332 us): the weights 222, the exponentials 289, the
+// conversion 316.
 //
 // Precision is that of the kernel for few rows (kv8.cu): float32 queries and
 // weights are two float16 pieces each, float16 queries one and their weights
@@ -445,8 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                     l *= f;
                 };
                 if constexpr (PP == 1) {
-                    // The maximum of the steps before serves as long as no weight is above 2^14 (float16 ends at 2^16);
-                    // looking for this step's first took a fifth of the time.
+                    // The maximum of the steps before serves as long as no weight is above 2^14 (float16 ends at 2^16); with
+                    // this step's looked for first the three prompts took 334 us in place of 298.
                     fresh = j == 0;
                     if (!fresh) {
                         sum = weigh(big);
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                         tm_st_wait();  // (stores of one thread have no order of their own)
                         sum = weigh(big);
                     }
-                } else {  // (two pieces leave no registers for weighing twice: 232 us for 194)
+                } else {  // (two pieces leave no registers for weighing twice: it spilled and was slower)
                     const float top = find();
                     fresh = __any_sync(kFull, top - m > 8.f);
                     if (fresh) raise(top);

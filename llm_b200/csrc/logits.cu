@@ -17,14 +17,23 @@
 // 0..18, bit 19 for the prompt's tokens, in bits 20..31 the place of the
 // token's bias (1..4095).  Counts are integers and of a token's biases the
 // last counts, so the order of the atomics does not matter.  The pass looks a
-// logit's word up and works out those that have one.  Bound by latency: a CTA
-// has about 10 K logits, so everything it reads first (logits, history,
-// biases, lengths) is asked for before the table is cleared, and there are
-// two barriers in all.  64 rows of 151936 float32 logits with histories of up to
-// 4096: 38 us, 2.1 TB/s, 32 % of the measured copy rate (20 us without a
-// history): 270 instructions for 128 logits, of which counting and the
-// divisions of single lanes take 4 us each.  One row: 5.6 us, latency.  The cluster's first CTA takes the largest of the CTAs'
-// maxima; the others do not wait for it.
+// logit's word up and works out those that have one.
+//
+// Bound by instructions, and by latency at the start of a round, which has at
+// most 11264 tokens of a CTA: what the round reads first (two vectors of logits
+// a thread, and in the first round the history, biases and lengths) is asked
+// for before the table is cleared, and there are two barriers in it and one
+// between rounds.  64 rows of 151936 float32 logits with histories of up to
+// 4096, in two rounds of 9504 tokens for each of 8 CTAs, so that the history is
+// read and counted twice: 35 us, 2.3 TB/s, 35 % of the measured copy rate (20 us
+// without a history; bfloat16 35 us too): 270 instructions for 128 logits, of
+// which counting and the divisions of single lanes take 4 us each.  64 rows of
+// 50256 take 17 us, of 50257, of which only every fourth is aligned to 16 bytes
+// and all go element by element, 18 (bfloat16 18 and 30).  One row of 49152: 5.5
+// us, latency.
+//
+// The cluster's first CTA takes the largest of the CTAs' maxima; the others do
+// not wait for it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
