@@ -273,7 +273,8 @@ typedef struct {
     int32_t table_stride;    /* entries of a table row */
     int32_t n_rows;          /* rows of the call's buffers */
     int32_t max_new;         /* no sequence has more rows than this; 0: not known (n_rows) */
-    int32_t max_len;         /* no sequence has more positions; 0: not known (table_stride * block) */
+    int32_t max_len;         /* no sequence has more positions; 0: not known (table_stride * block).  The attention cuts
+                              * its work by this bound, so a close one is faster */
 } llmb_kv8_batch;
 
 /* Writes the rows of k and v (n_rows rows of [kv_heads][head_dim] elements

@@ -362,7 +362,7 @@ struct Place {
 // Bound, B200: one sequence of 131071 positions (32 heads on 8, size 128,
 // e4m3, bfloat16 rows) 66 us with its join, 4.1 TB/s, 63 % of the measured copy
 // rate: copies in flight and the ends of the one wave.  64 sequences of up to
-// 2048 (9 heads on 3, size 64, int8, float32) 16.5 us, 2.0 TB/s: 324
+// 2048 (9 heads on 3, size 64, int8, float32) 17.7 us, 1.9 TB/s: 324
 // instructions a group and the sequences' different lengths.  300 positions of
 // one sequence 6 us: latency.
 //
@@ -387,8 +387,8 @@ constexpr int kPieces<__nv_bfloat16> = 1;
 
 // Groups of a warp in flight, as many as four CTAs an SM have room for (a group is 32 HD bytes), and their bytes.
 __host__ __device__ constexpr int att_depth(int hd) { return hd == 64 ? 6 : 3; }
-// Groups worked on at once: two where the registers of four CTAs an SM hold them (us, with one / with two: 64 sequences 16.6 /
-// 16.4, the window of 4000 in bfloat16 15.4 / 14.8, a chunk of 64 behind 1920 17.0 / 16.4).
+// Groups worked on at once: two where the registers of four CTAs an SM hold them (us with one / with two, the cache in L2: 64
+// sequences 16.6 / 16.4, 33 with a window of 4000 in bfloat16 15.4 / 14.8, a chunk of 64 behind 1920 17.0 / 16.4).
 __host__ __device__ constexpr int att_groups(int hd, int nb) { return hd == 64 && nb == 1 ? 2 : 1; }
 __host__ __device__ constexpr int att_smem(int hd) { return kAttWarps * att_depth(hd) * 32 * hd; }
 

@@ -23,8 +23,8 @@
 // a step's maximum otherwise).
 //
 // Three prompts of up to 1023 tokens behind 4000 positions (32 heads on 8, size
-// 128, int8): bfloat16 rows 300 us, 634 TFLOP/s, 38 % of the measured bf16
-// rate, float16 437, float32 708; 360 tiles are 2.4 waves.  The chain of one
+// 128, int8): bfloat16 rows 301 us, 632 TFLOP/s, 38 % of the measured bf16
+// rate, float16 428, float32 707; 360 tiles are 2.4 waves.  The chain of one
 // tile, softmax and then its two products, bounds a step, then shared memory's
 // rate: 192 KB of operands, 64 KB of float16 stored and 64 KB of copies a step
 // of two tiles.  Left out one at a time, when a step's maximum was still looked

@@ -25,11 +25,11 @@
 // for before the table is cleared, and there are two barriers in it and one
 // between rounds.  64 rows of 151936 float32 logits with histories of up to
 // 4096, in two rounds of 9504 tokens for each of 8 CTAs, so that the history is
-// read and counted twice: 35 us, 2.3 TB/s, 35 % of the measured copy rate (20 us
-// without a history; bfloat16 35 us too): 270 instructions for 128 logits, of
+// read and counted twice: 37 us, 2.2 TB/s, 33 % of the measured copy rate (22 us
+// without a history; bfloat16 37 us too): 270 instructions for 128 logits, of
 // which counting and the divisions of single lanes take 4 us each.  64 rows of
-// 50256 take 17 us, of 50257, of which only every fourth is aligned to 16 bytes
-// and all go element by element, 18 (bfloat16 18 and 30).  One row of 49152: 5.5
+// 50256 take 19 us, of 50257, of which only every fourth is aligned to 16 bytes
+// and all go element by element, 21 (bfloat16 20 and 31).  One row of 49152: 5.4
 // us, latency.
 //
 // The cluster's first CTA takes the largest of the CTAs' maxima; the others do
