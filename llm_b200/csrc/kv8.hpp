@@ -126,8 +126,8 @@ __device__ __forceinline__ bool kv8_query_scale(uint32_t m, float &up, float &do
 // 2^121) mv is in [1, 2), or down to 2^-8 at the least ones: 2^-ex times the largest weight (2^6) must leave the sum of 2^21
 // positions finite, and weights times 2^-8 still have their 22 bits.  A group whose scale is 0 or smaller than those counts
 // in the softmax's sum, and its weights' size must not hide those of values that are not 0 (float16 ends 2^31 below the
-// largest): it takes the least exponent of the walk so far (low), or before the walk has one kKv8ZeroExp, from which any
-// that is met later is in reach.
+// largest): it takes the least exponent of the walk so far (low), or before the walk has one kKv8ZeroExp, from which any up
+// to 2^60 that is met later is in reach.
 constexpr int kKv8LeastScale = -109, kKv8LeastExp = -101, kKv8ZeroExp = -64, kKv8NoExp = 0x7fffffff;
 __device__ __forceinline__ float kv8_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ int kv8_v_scale(float vs, float &mv, int &low) {

@@ -23,8 +23,8 @@
 // a step's maximum otherwise).
 //
 // Three prompts of up to 1023 tokens behind 4000 positions (32 heads on 8, size
-// 128, int8): bfloat16 rows 301 us, 632 TFLOP/s, 38 % of the measured bf16
-// rate, float16 428, float32 707; 360 tiles are 2.4 waves.  The chain of one
+// 128, int8): bfloat16 rows 299 us, 635 TFLOP/s, 38 % of the measured bf16
+// rate, float16 437, float32 707; 360 tiles are 2.4 waves.  The chain of one
 // tile, softmax and then its two products, bounds a step, then shared memory's
 // rate: 192 KB of operands, 64 KB of float16 stored and 64 KB of copies a step
 // of two tiles.  Left out one at a time, when a step's maximum was still looked
@@ -64,8 +64,8 @@ template <class T> constexpr int kPPieces = 2;
 template <> constexpr int kPPieces<__nv_bfloat16> = 1;
 
 // What 16 positions share: K's scale; V's scale = mv 2^lv, with 2^-lv in the unit of the weights' sums.  bfloat16 rows, whose
-// precision leaves room for the rounding of a logarithm, have all of the scale in lv, and mv is not used; a scale that has
-// no logarithm, or is below all that append makes, makes the group's values 0 for them as they are stored for the products.
+// precision leaves room for the rounding of a logarithm, have all of the scale in lv, and mv is not used; where a scale has
+// no logarithm, or is below all that append makes, the group's values are 0 for them: zeros are stored in place of its copy.
 struct Group {
     float ks, lv, mv, unlv;
 };
@@ -94,7 +94,7 @@ struct Layout {
 
 struct Bars {
     uint64_t full[4], empty[4], raw[8], free[8], group[8], s[2], p[2], q[2], o[2], done;
-    uint32_t tmem, fail, none[8];  // none: a step's groups whose values are 0, a bit each
+    uint32_t tmem, fail;
 };
 static_assert(sizeof(Bars) <= 384, "the barriers' space");
 
@@ -570,12 +570,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
             uint4 x[NP];
 #pragma unroll
             for (int n = 0; n < NP; ++n) x[n] = *reinterpret_cast<const uint4 *>(src + n * 2048);
-            if (PP == 1 && (i & 1)) {
-                if (const uint32_t none = bar.none[(i >> 1) & 7])  // (written before the wait for these copies began)
-#pragma unroll
-                    for (int n = 0; n < NP; ++n)
-                        if (none >> ((key0 + n * (128 / PC)) >> 4) & 1) x[n] = make_uint4(0, 0, 0, 0);
-            }
             __syncwarp();
             if (lane == 0) bar_arrive(&bar.free[i % D]);
 #pragma unroll
@@ -673,29 +667,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_chunk(const Kv8 c, const Kv
                 const int per = c.block >> 4, in_block = ((lo + j * kKeys) >> 4) + lane & (per - 1);
                 const bool first = b >= 0 && (lane == 0 || in_block == 0);
                 const int n = min(min(per - in_block, 8 - lane), ((hi - lo - j * kKeys + 15) >> 4) - lane);
+                const bool scaled = vs >= kv8_pow2(kKv8LeastScale) && vs <= FLT_MAX;
                 const uint32_t bytes = 16 * HD * __popc(__ballot_sync(kFull, b >= 0));
                 for (int i = 2 * j; i < 2 * j + 2; ++i) {
                     ok = i < D || bar_wait(&bar.free[i % D], (i / D - 1) & 1, fail);
                     if (!(ok = __all_sync(kFull, ok))) break;
-                    if (PP == 1 && (i & 1)) {
-                        const uint32_t none = __ballot_sync(kFull, b >= 0 && !(vs >= kv8_pow2(kKv8LeastScale) && vs <= FLT_MAX));
-                        if (lane == 0) bar.none[j & 7] = none;
-                    }
-                    if (lane == 0) bar_expect(&bar.raw[i % D], bytes);
+                    // blocks whose values are 0, whatever their bytes
+                    const uint32_t none = PP == 1 && (i & 1) ? __ballot_sync(kFull, b >= 0 && !scaled) : 0;
+                    for (uint32_t left = none; left; left &= left - 1)
+                        for (int k = lane; k < HD; k += 32)
+                            *reinterpret_cast<uint4 *>(smem + L::raw + (i % D) * 128 * HD + (__ffs(left) - 1) * 16 * HD + 16 * k) =
+                                make_uint4(0, 0, 0, 0);
+                    if (none) fence_async();  // later copies come after these stores
                     __syncwarp();
-                    if (first) bulk(smem + L::raw + (i % D) * 128 * HD + lane * 16 * HD, (i & 1 ? c.v : c.k) + off, n * 16 * HD, &bar.raw[i % D]);
+                    if (lane == 0) bar_expect(&bar.raw[i % D], bytes - 16 * HD * __popc(none));
+                    __syncwarp();
+                    if (first && !(none >> lane & 1))
+                        bulk(smem + L::raw + (i % D) * 128 * HD + lane * 16 * HD, (i & 1 ? c.v : c.k) + off, n * 16 * HD, &bar.raw[i % D]);
                     sent = i + 1;
                 }
                 if (!ok) break;
                 // The groups' scales.  Their place was last read in step j - 8, which was over: this step's V is copied to
                 // where V of step j - copies / 2 was, after that was stored to a slot, after the products that used the
                 // slot before, of a step j - 6 at the earliest, and so the weights of the step before that, were done.
-                // (So was the converters' look at none: they had V of step j - copies / 2 by then.)
                 Group g = {0.f, -INFINITY, 0.f, 0.f};  // no block: -inf as a score
                 const int ex = kv8_v_scale(vs, g.mv, low);
                 if (b >= 0) {
                     g.ks = ks, g.lv = (float)ex, g.unlv = kv8_pow2(-ex) * SU;
-                    if (PP == 1 && vs >= kv8_pow2(kKv8LeastScale) && vs <= FLT_MAX) g.lv = log2f(vs), g.unlv = SU / vs;
+                    if (PP == 1 && scaled) g.lv = log2f(vs), g.unlv = SU / vs;
                 }
                 if (lane < 8) groups[(j & 7) * 8 + lane] = g;
                 __syncwarp();
